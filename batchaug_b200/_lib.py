@@ -34,11 +34,17 @@ BA_SHIFT_SAFE = 0x1
 BA_RESCALE_MINV, BA_RESCALE_MAXV, BA_RESCALE_CHANNEL, BA_RESCALE_FACTOR = 0x1, 0x2, 0x4, 0x8
 BA_RESCALE_GIVEN = 0x10
 
+BA_CHANNELS_FIRST, BA_CHANNELS_LAST = 0, 1
+BA_ACT_NONE, BA_ACT_RELU, BA_ACT_LEAKY_RELU, BA_ACT_SILU, BA_ACT_GELU = 0, 1, 2, 3, 4
+BA_DROPOUT_CHANNEL, BA_DROPOUT_RESCALE = 0x1, 0x2
+
 BA_SMOOTH_ZEROS, BA_SMOOTH_REFLECT, BA_SMOOTH_REPLICATE = 0, 1, 2
 
 MODES = {"bilinear": BA_BILINEAR, "nearest": BA_NEAREST}
 SMOOTH_PADS = {None: BA_SMOOTH_ZEROS, "constant": BA_SMOOTH_ZEROS, "reflect": BA_SMOOTH_REFLECT,
                "replicate": BA_SMOOTH_REPLICATE}
+ACTIVATIONS = {None: BA_ACT_NONE, "none": BA_ACT_NONE, "relu": BA_ACT_RELU,
+               "leaky_relu": BA_ACT_LEAKY_RELU, "silu": BA_ACT_SILU, "gelu": BA_ACT_GELU}
 PADDINGS = {"zeros": BA_PAD_ZEROS, "border": BA_PAD_BORDER, "reflection": BA_PAD_REFLECTION}
 
 _P = ctypes.c_void_p
@@ -86,6 +92,23 @@ class LowresDesc(ctypes.Structure):
                 ("max_zoom", ctypes.c_double)]
 
 
+class DropoutDesc(ctypes.Structure):
+    _fields_ = [("src", _P), ("dst", _P), ("batch", _I64), ("channels", _I64), ("H", _I64),
+                ("W", _I64), ("D", _I64), ("dtype", _I32), ("layout", _I32), ("flags", _I32),
+                ("p", ctypes.c_float), ("p_elem", _P), ("mask", _P), ("seed", _U64),
+                ("seed_dev", _P), ("elem_offset", _U64)]
+
+
+class NormDesc(ctypes.Structure):
+    _fields_ = [("x", _P), ("dy", _P), ("out", _P), ("weight", _P), ("bias", _P),
+                ("dweight", _P), ("dbias", _P), ("stats", _P), ("batch", _I64),
+                ("channels", _I64), ("H", _I64), ("W", _I64), ("D", _I64), ("groups", _I64),
+                ("dtype", _I32), ("layout", _I32), ("param_dtype", _I32), ("activation", _I32),
+                ("eps", ctypes.c_float), ("slope", ctypes.c_float), ("p", ctypes.c_float),
+                ("reserved", _I32), ("p_elem", _P), ("seed", _U64), ("seed_dev", _P),
+                ("elem_offset", _U64)]
+
+
 INTERP_MODES = {"nearest": 0, "nearest-exact": 1, "trilinear": 2, "area": 3}
 
 
@@ -110,6 +133,10 @@ SIGNATURES = {
     "ba_elastic_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
     "ba_elastic_grid": (_I32, [_P, _U64, _U64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
                                ctypes.c_size_t, _P]),
+    "ba_dropout": (_I32, [ctypes.POINTER(DropoutDesc), _P]),
+    "ba_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormDesc), _I32]),
+    "ba_norm_forward": (_I32, [ctypes.POINTER(NormDesc), _P, ctypes.c_size_t, _P]),
+    "ba_norm_backward": (_I32, [ctypes.POINTER(NormDesc), _P, ctypes.c_size_t, _P]),
     "ba_host_uniform": (None, [_U64, ctypes.c_uint32, _U64, _I64, _I64, _P]),
     "ba_host_rand_affine": (None, [_P, _I64, _I64, ctypes.c_float, _P, _P, _P, ctypes.c_uint32,
                                    ctypes.c_uint32, _I64, _I64, _I64, _P, _P, _P]),

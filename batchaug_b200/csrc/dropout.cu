@@ -1,0 +1,138 @@
+// ba_dropout: one read and one write of the tensor, the mask drawn from the
+// counter as it goes (dropout.cuh).
+#include "feature.cuh"
+
+namespace ba {
+namespace {
+
+struct DropoutArgs {
+  const void* src;
+  void* dst;
+  Feat f;
+  DropArgs drop;
+  int32_t channelwise;
+};
+
+template <int DT, int VEC>
+__global__ void __launch_bounds__(FEAT_THREADS)
+    dropout_last(const __grid_constant__ DropoutArgs a) {
+  const LastPlace p = last_place<VEC>(a.f);
+  if (!p.on) return;
+  const DropRate dr = drop_rate(a.drop, p.b);
+  const int64_t base = p.b * a.f.S * a.f.C + p.c;
+  uint32_t keep[VEC];
+  if (a.channelwise) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) keep[i] = drop_keep_channel(dr, p.c + i) ? 0xFFu : 0u;
+  }
+  for (int64_t r = p.r0 + p.ty * 8; r < p.r1; r += p.nty * 8) {
+    Raw<DT, VEC> rx[8];
+    const int n = (int)min((int64_t)8, p.r1 - r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) rx[j] = raw_load<DT, VEC>(a.src, base + (r + j) * a.f.C);
+    if (!a.channelwise) last_keep<VEC>(a.f, dr, p.c, r, keep);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) {
+        float v[VEC];
+        raw_unpack<DT, VEC>(rx[j], v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = (keep[i] >> j) & 1u ? v[i] * dr.scale : 0.0f;
+        raw_store<DT, VEC>(a.dst, base + (r + j) * a.f.C, raw_pack<DT, VEC>(v));
+      }
+  }
+}
+
+template <int DT, int VEC>
+__global__ void __launch_bounds__(FEAT_THREADS)
+    dropout_first(const __grid_constant__ DropoutArgs a) {
+  FirstPlace p;
+  if (!first_place(a.f, p)) return;
+  const DropRate dr = drop_rate(a.drop, p.b);
+  constexpr int FLIGHT = 4;
+  const uint32_t row = a.channelwise ? (drop_keep_channel(dr, p.c) ? 0xFFu : 0u) : 0u;
+  for (int64_t s = p.s0; s < p.s1; s += FEAT_TILE * FLIGHT) {
+    FirstTile<DT, VEC> t[FLIGHT];
+#pragma unroll
+    for (int u = 0; u < FLIGHT; ++u) first_load<DT, VEC>(a.src, p, s + u * FEAT_TILE, t[u]);
+#pragma unroll
+    for (int u = 0; u < FLIGHT; ++u) {
+      const int64_t su = s + u * FEAT_TILE;
+      if (su < p.s1) {
+        const uint32_t keep = a.channelwise ? row : first_keep<VEC>(a.f, dr, p, su);
+        float v[8];
+        first_unpack<DT, VEC>(t[u], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (keep >> i) & 1u ? v[i] * dr.scale : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j += VEC)
+          if (su + first_at<VEC>(p.lane, j) < p.s1)
+            raw_store<DT, VEC>(a.dst, p.base + su + first_at<VEC>(p.lane, j),
+                               raw_pack<DT, VEC>(v + j));
+      }
+    }
+  }
+}
+
+template <int DT, int VEC>
+void launch(const DropoutArgs& a, bool last, dim3 grid, cudaStream_t st) {
+  if (last)
+    dropout_last<DT, VEC><<<grid, FEAT_THREADS, 0, st>>>(a);
+  else if constexpr (DT == BA_F32 || VEC != 4)
+    dropout_first<DT, VEC><<<grid, FEAT_THREADS, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace ba
+
+extern "C" ba_status ba_dropout(const ba_dropout_desc* desc, ba_stream_t stream) {
+  using namespace ba;
+  clear_error();
+  BA_REQUIRE(desc != nullptr, "ba_dropout: desc is NULL");
+  const ba_dropout_desc& d = *desc;
+  ba_status st = feat_check("ba_dropout", d.batch, d.channels, d.H, d.W, d.D, d.dtype, d.layout);
+  if (st != BA_OK) return st;
+  BA_REQUIRE((d.flags & ~(BA_DROPOUT_CHANNEL | BA_DROPOUT_RESCALE)) == 0,
+             "ba_dropout: unknown flags 0x%x", d.flags);
+  BA_REQUIRE(d.p_elem != nullptr || (d.p >= 0.0f && d.p <= 1.0f),
+             "ba_dropout: p=%g not in [0, 1]", (double)d.p);
+  const int64_t S = d.H * d.W * d.D;
+  if (d.batch * d.channels * S == 0) return BA_OK;
+  const size_t esz = d.dtype == BA_BF16 ? 2 : 4;
+  const size_t bytes = (size_t)(d.batch * d.channels * S) * esz;
+  BA_REQUIRE(d.src && d.dst, "ba_dropout: NULL src or dst");
+  BA_REQUIRE((uintptr_t)d.src % esz == 0 && (uintptr_t)d.dst % esz == 0,
+             "ba_dropout: pointers not aligned to the element size");
+  BA_REQUIRE((uintptr_t)d.p_elem % 4 == 0 && (uintptr_t)d.seed_dev % 8 == 0,
+             "ba_dropout: p_elem or seed_dev not aligned");
+  BA_REQUIRE(d.src == d.dst || !feat_overlap(d.src, d.dst, bytes),
+             "ba_dropout: dst partially overlaps src");
+  DropoutArgs a;
+  a.src = d.src;
+  a.dst = d.dst;
+  const void* ptrs[2] = {d.src, d.dst};
+  a.f = feat_plan(d.batch, d.channels, S, d.dtype, d.layout, ptrs, 2);
+  a.drop = {d.p, d.p_elem, d.mask, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
+            d.elem_offset, (d.flags & BA_DROPOUT_RESCALE) ? 1 : 0};
+  a.channelwise = (d.flags & BA_DROPOUT_CHANNEL) ? 1 : 0;
+  dim3 grid;
+  st = feat_grid("ba_dropout", a.f, d.layout, &grid);
+  if (st != BA_OK) return st;
+  const bool last = d.layout == BA_CHANNELS_LAST;
+  cudaStream_t cs = (cudaStream_t)stream;
+  if (d.dtype == BA_BF16) {
+    if (a.f.vec == 8)
+      launch<BA_BF16, 8>(a, last, grid, cs);
+    else if (a.f.vec == 4)
+      launch<BA_BF16, 4>(a, last, grid, cs);
+    else
+      launch<BA_BF16, 1>(a, last, grid, cs);
+  } else {
+    if (a.f.vec == 4)
+      launch<BA_F32, 4>(a, last, grid, cs);
+    else
+      launch<BA_F32, 1>(a, last, grid, cs);
+  }
+  return check_launch("ba_dropout");
+}

@@ -1,0 +1,123 @@
+// Counter-based dropout bits, shared by the dropout kernels, the group norm's
+// epilogue and the intensity chain.  The mask is never stored: every pass
+// that needs it draws it again from the counter.
+//
+// Voxel s of channel c of global element e owns a 32-bit number r, and stays
+// iff r >= ceil(p * 2^32), so it is dropped with probability p to 2^-32.  The
+// numbers of 8 consecutive voxels of a channel come from one Philox block:
+//   q = c * ceil(S / 8) + s / 8,
+//   counter (q, e, e >> 32, STREAM | q >> 32), key = seed;
+// its four words are eight 16-bit halves (low half first), the high halves
+// of the eight numbers.  The low halves are the same block on a second
+// stream, and are drawn only when a high half equals the threshold's high
+// half and the threshold's low half is not zero: one block in 8,192 for a
+// threshold that needs it.  So eight decisions of 32 bits cost one Philox
+// block (ten rounds, ~60 issue slots), not two; a 16-byte vector of bf16 then
+// costs fewer issue slots than its HBM time allows.
+//
+// The bits depend on (seed, global element, channel, voxel) alone: not on
+// the memory layout, the launch shape or the batch's sharding.
+#pragma once
+
+#include "ba_common.cuh"
+#include "philox.cuh"
+
+namespace ba {
+
+constexpr uint32_t STREAM_DROP = 0x44500000u;             // voxels, high halves
+constexpr uint32_t STREAM_DROP_LOW = 0x44510000u;         // voxels, low halves
+constexpr uint32_t STREAM_DROP_CHANNEL = 0x44520000u;     // channels, high halves
+constexpr uint32_t STREAM_DROP_CHANNEL_LOW = 0x44530000u; // channels, low halves
+
+// The drop rate's source and the generator's key, as the host passes them.
+struct DropArgs {
+  float p;                 // the rate when p_elem is NULL
+  const float* p_elem;     // (B,) rates
+  const uint8_t* mask;     // (B,) 0/1: elements to drop in, NULL = every one
+  uint32_t seed_lo, seed_hi;
+  const uint64_t* seed_dev;  // the key in device memory, NULL: seed_lo / seed_hi
+  uint64_t elem_offset;
+  int rescale;             // scale what stays by 1 / (1 - p)
+};
+
+// An element's rate, resolved.
+struct DropRate {
+  uint32_t hi, lo;    // halves of the threshold; hi == 0x10000: nothing stays
+  uint32_t k0, k1;    // Philox key
+  uint32_t e_lo, e_hi;
+  float scale;        // of what stays
+};
+
+__device__ __forceinline__ DropRate drop_rate(const DropArgs& a, int64_t b) {
+  DropRate r;
+  const bool on = a.mask == nullptr || a.mask[b] != 0;
+  float p = a.p_elem != nullptr ? a.p_elem[b] : a.p;
+  p = (on && p > 0.0f) ? p : 0.0f;  // NaN counts as 0
+  r.scale = (a.rescale && on) ? (p < 1.0f ? __fdiv_rn(1.0f, 1.0f - p) : 0.0f) : 1.0f;
+  // p * 2^32 is exact; below 1 it is at most 2^32 - 2^8
+  const uint32_t t = p < 1.0f ? __float2uint_ru(p * 4294967296.0f) : 0u;
+  r.hi = p < 1.0f ? t >> 16 : 0x10000u;
+  r.lo = p < 1.0f ? t & 0xFFFFu : 0u;
+  if (a.seed_dev != nullptr) {
+    const uint64_t s = *a.seed_dev;
+    r.k0 = (uint32_t)s;
+    r.k1 = (uint32_t)(s >> 32);
+  } else {
+    r.k0 = a.seed_lo;
+    r.k1 = a.seed_hi;
+  }
+  const uint64_t e = a.elem_offset + (uint64_t)b;
+  r.e_lo = (uint32_t)e;
+  r.e_hi = (uint32_t)(e >> 32);
+  return r;
+}
+
+__device__ __forceinline__ U4 drop_block(const DropRate& r, uint64_t q, uint32_t stream) {
+  const U4 ctr = {(uint32_t)q, r.e_lo, r.e_hi, stream | (uint32_t)(q >> 32)};
+  return philox4x32_10(ctr, r.k0, r.k1);
+}
+
+// Bit i set: number i of block q stays.
+__device__ __forceinline__ uint32_t drop_keep8(const DropRate& r, uint64_t q,
+                                               uint32_t stream = STREAM_DROP,
+                                               uint32_t stream_low = STREAM_DROP_LOW) {
+  if (r.hi == 0u && r.lo == 0u) return 0xFFu;
+  if (r.hi > 0xFFFFu) return 0u;
+  const U4 b = drop_block(r, q, stream);
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+  const uint32_t t = r.hi << 16;
+  uint32_t keep = 0u, tie = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    keep |= (w[j] << 16 >= t ? 1u : 0u) << (2 * j);
+    keep |= (w[j] >= t ? 1u : 0u) << (2 * j + 1);
+  }
+  if (r.lo != 0u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      tie |= ((w[j] & 0xFFFFu) == r.hi ? 1u : 0u) << (2 * j);
+      tie |= (w[j] >> 16 == r.hi ? 1u : 0u) << (2 * j + 1);
+    }
+    if (tie != 0u) {
+      const U4 l = drop_block(r, q, stream_low);
+      const uint32_t v[4] = {l.x, l.y, l.z, l.w};
+      uint32_t ge = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ge |= ((v[j] & 0xFFFFu) >= r.lo ? 1u : 0u) << (2 * j);
+        ge |= (v[j] >> 16 >= r.lo ? 1u : 0u) << (2 * j + 1);
+      }
+      keep &= ~tie | ge;
+    }
+  }
+  return keep;
+}
+
+// Whether channel c of the element stays (channelwise dropout).
+__device__ __forceinline__ bool drop_keep_channel(const DropRate& r, int64_t c) {
+  const uint32_t k =
+      drop_keep8(r, (uint64_t)c >> 3, STREAM_DROP_CHANNEL, STREAM_DROP_CHANNEL_LOW);
+  return (k >> (c & 7)) & 1u;
+}
+
+}  // namespace ba

@@ -406,6 +406,214 @@ def elastic_grid(shape, taps, magnitude, *, u=None, seed=0, elem_offset=0,
     return grid
 
 
+# ---------------------------------------------------------------------------
+# Feature maps: dropout and group norm (differentiable)
+# ---------------------------------------------------------------------------
+
+def _feature_map(x: torch.Tensor, name: str):
+    """``x`` dense in one of the two layouts the kernels take, and which: a
+    (B,C,H,W,D) tensor contiguous as named or in torch.channels_last_3d is
+    taken as it is, any other strides are copied to the former."""
+    L.require_cuda(x, name)
+    if x.dim() != 5:
+        raise ValueError(f"expected a (B,C,H,W,D) tensor, got shape {tuple(x.shape)}")
+    if x.is_contiguous():
+        return x, L.BA_CHANNELS_FIRST
+    if x.is_contiguous(memory_format=torch.channels_last_3d):
+        return x, L.BA_CHANNELS_LAST
+    return x.contiguous(), L.BA_CHANNELS_FIRST
+
+
+def _like(t: torch.Tensor, x: torch.Tensor, layout: int) -> torch.Tensor:
+    """``t`` (a gradient) with x's dtype and layout."""
+    if t.dtype != x.dtype:
+        t = t.to(x.dtype)
+    return t.contiguous(memory_format=torch.channels_last_3d if layout == L.BA_CHANNELS_LAST
+                        else torch.contiguous_format)
+
+
+def _drop_params(x: torch.Tensor, p, seed, name: str):
+    """Checked (p, p_elem, seed, seed_dev): a probability in [0, 1] or a (B,)
+    tensor of them, and an integer seed or an int64 CUDA tensor holding one."""
+    p_elem = seed_dev = None
+    if isinstance(p, torch.Tensor):
+        if p.numel() != x.shape[0]:
+            raise ValueError(f"{name}: p has {p.numel()} values for a batch of {x.shape[0]}")
+        p_elem = p.detach().to(device=x.device, dtype=torch.float32).reshape(-1).contiguous()
+        p = 0.0
+    else:
+        p = float(p)
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"{name}: p={p} is not a probability")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+            raise ValueError(f"{name}: a seed tensor must be one int64 on {x.device}")
+        seed_dev, seed = seed, 0
+    elif seed is None:
+        if p_elem is not None or p > 0.0:
+            raise ValueError(f"{name}: dropout needs a seed")
+        seed = 0
+    return p, p_elem, int(seed) & 0xFFFFFFFFFFFFFFFF, seed_dev
+
+
+def _on(device: torch.device):
+    """The device made current, when it is another one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _dropout_call(x, layout, spec, p_elem, mask, seed_dev, out=None):
+    out = torch.empty_like(x) if out is None else out
+    p, seed, elem_offset, flags = spec
+    B, C, H, W, D = x.shape
+    d = L.DropoutDesc(x.data_ptr(), out.data_ptr(), B, C, H, W, D, L.dtype_code(x), layout, flags,
+                      p, L.ptr(p_elem), L.ptr(mask), seed, L.ptr(seed_dev), elem_offset)
+    with _on(x.device):
+        tok = _timing.begin("ba_dropout", 2 * x.numel() * x.element_size(), x.device)
+        L.check(L.lib.ba_dropout(ctypes.byref(d), L.stream_ptr(x.device)), "ba_dropout")
+        _timing.end(tok)
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, layout, spec, p_elem, mask, seed_dev):
+        ctx.layout, ctx.spec = layout, spec
+        ctx.save_for_backward(p_elem, mask, seed_dev)
+        return _dropout_call(x, layout, spec, p_elem, mask, seed_dev)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        # the same draw on the gradient
+        dx = _dropout_call(_like(dy, dy, ctx.layout), ctx.layout, ctx.spec, *ctx.saved_tensors)
+        return dx, None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
+            channelwise: bool = False, rescale: bool = True) -> torch.Tensor:
+    """Zero each voxel of x (B,C,H,W,D) with probability ``p`` and scale the
+    others by 1 / (1 - p) (``rescale``); ``channelwise`` draws once for each
+    (element, channel).  Differentiable; the mask is never stored, the
+    backward pass draws it again.
+
+    ``p``: a number, or a (B,) tensor with a rate for each element.  ``mask``
+    (B,): elements left as they are where false.  ``seed``: an integer, or a
+    CUDA int64 tensor of one value that the kernel reads when it runs, so a
+    captured graph draws other bits after the caller has changed it (the
+    backward pass must see the value that the forward pass saw).  The bits
+    depend on (seed, elem_offset + element, channel, voxel) only, not on
+    the memory layout, which the result shares with x."""
+    x, layout = _feature_map(x, "x")
+    L.dtype_code(x)
+    p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "dropout")
+    m = _dev_mask(mask, x.shape[0], x.device)
+    flags = (L.BA_DROPOUT_CHANNEL if channelwise else 0) | (L.BA_DROPOUT_RESCALE if rescale else 0)
+    spec = (p, seed, int(elem_offset), flags)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dropout.apply(x, layout, spec, p_elem, m, seed_dev)
+    return _dropout_call(x, layout, spec, p_elem, m, seed_dev)
+
+
+def _norm_desc(x, layout, spec, weight, bias, p_elem, seed_dev, stats):
+    groups, act, eps, slope, p, seed, elem_offset = spec
+    B, C, H, W, D = x.shape
+    param = weight if weight is not None else bias
+    return L.NormDesc(x.data_ptr(), None, None, L.ptr(weight), L.ptr(bias), None, None,
+                      stats.data_ptr(), B, C, H, W, D, groups, L.dtype_code(x), layout,
+                      L.BA_F32 if param is None else L.dtype_code(param), act, eps, slope, p, 0,
+                      L.ptr(p_elem), seed, L.ptr(seed_dev), elem_offset)
+
+
+def _norm_run(d, backward, name, nbytes, device):
+    with _on(device):
+        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(d), backward)
+        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        tok = _timing.begin(name, nbytes, device)
+        fn = L.lib.ba_norm_backward if backward else L.lib.ba_norm_forward
+        L.check(fn(ctypes.byref(d), L.ptr(ws), size, L.stream_ptr(device)), name)
+        _timing.end(tok)
+
+
+def _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev):
+    y = torch.empty_like(x)
+    stats = torch.empty((x.shape[0], spec[0], 2), dtype=torch.float32, device=x.device)
+    d = _norm_desc(x, layout, spec, weight, bias, p_elem, seed_dev, stats)
+    d.out = y.data_ptr()
+    _norm_run(d, 0, "ba_norm_forward", 2 * x.numel() * x.element_size(), x.device)
+    return y, stats
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, layout, spec, p_elem, seed_dev):
+        y, stats = _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev)
+        ctx.layout, ctx.spec = layout, spec
+        ctx.save_for_backward(x, weight, bias, p_elem, seed_dev, stats)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, p_elem, seed_dev, stats = ctx.saved_tensors
+        dy = _like(dy, x, ctx.layout)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
+        d = _norm_desc(x, ctx.layout, ctx.spec, weight, bias, p_elem, seed_dev, stats)
+        d.dy, d.out, d.dweight, d.dbias = dy.data_ptr(), L.ptr(dx), L.ptr(dw), L.ptr(db)
+        _norm_run(d, 1, "ba_norm_backward", 3 * x.numel() * x.element_size(), x.device)
+        return dx, dw, db, None, None, None, None
+
+
+def _norm_param(t, x, name):
+    if t is None:
+        return None
+    if t.device != x.device:
+        raise ValueError(f"group_norm: {name} is on {t.device}, x on {x.device}")
+    if t.dim() != 1 or t.shape[0] != x.shape[1]:
+        raise ValueError(f"group_norm: {name} must be ({x.shape[1]},), got {tuple(t.shape)}")
+    L.dtype_code(t)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps: float = 1e-5,
+               activation=None, negative_slope: float = 0.01, p=0.0, seed=None,
+               elem_offset: int = 0) -> torch.Tensor:
+    """dropout(activation(group_norm(x) * weight + bias)) of x (B,C,H,W,D),
+    each group of C / num_groups consecutive channels of an element
+    normalised by its own mean and biased variance.  Differentiable in x,
+    weight and bias.
+
+    ``activation``: None (or "none"), "relu", "leaky_relu" (with
+    ``negative_slope``), "silu" or "gelu" (exact).  ``weight`` and ``bias``
+    (C,), float32 or bfloat16 (the same for both), or None.  ``p``, ``seed``
+    and ``elem_offset``: as in :func:`dropout`, rescaled; no dropout by
+    default.  x may be contiguous or in torch.channels_last_3d, and the
+    result is laid out as it is."""
+    x, layout = _feature_map(x, "x")
+    L.dtype_code(x)
+    num_groups = int(num_groups)
+    if num_groups < 1 or x.shape[1] % num_groups:
+        raise ValueError(f"group_norm: {num_groups} groups do not divide {x.shape[1]} channels")
+    if activation not in L.ACTIVATIONS:
+        raise ValueError(f"unsupported activation {activation!r} (expected one of "
+                         f"{[a for a in L.ACTIVATIONS if a]})")
+    weight, bias = _norm_param(weight, x, "weight"), _norm_param(bias, x, "bias")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "group_norm")
+    spec = (num_groups, L.ACTIVATIONS[activation], float(eps), float(negative_slope), p, seed,
+            int(elem_offset))
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNorm.apply(x, weight, bias, layout, spec, p_elem, seed_dev)
+    return _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev)[0]
+
+
 def host_rand_affine(u, prob, a, b, c, present, groups, spatial_shape, mask, affine, theta):
     """ba_host_rand_affine into the given numpy outputs (mask u8 (B,),
     affine and theta (B,4,4) float32)."""

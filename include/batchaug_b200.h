@@ -265,6 +265,101 @@ BA_API ba_status ba_minmax(const void* x, int32_t dtype, int64_t n_groups, int64
                     float* stats, ba_stream_t stream);
 
 /* ---------------------------------------------------------------------- */
+/* Feature maps: dropout and group norm                                    */
+/* ---------------------------------------------------------------------- */
+
+/* How a (B, C, H, W, D) tensor lies in memory: as named, or with the channels
+ * innermost (torch.channels_last_3d). */
+typedef enum ba_layout { BA_CHANNELS_FIRST = 0, BA_CHANNELS_LAST = 1 } ba_layout;
+
+typedef enum ba_activation {
+  BA_ACT_NONE = 0,
+  BA_ACT_RELU = 1,
+  BA_ACT_LEAKY_RELU = 2, /* z < 0 ? slope * z : z */
+  BA_ACT_SILU = 3,       /* z / (1 + exp(-z)) */
+  BA_ACT_GELU = 4        /* z * Phi(z), Phi the normal distribution function */
+} ba_activation;
+
+/* ba_dropout_desc.flags */
+#define BA_DROPOUT_CHANNEL 0x1 /* one draw for each (element, channel) */
+#define BA_DROPOUT_RESCALE 0x2 /* what stays is scaled by 1 / (1 - p) */
+
+/*
+ * Dropout from a counter-based generator; no mask is stored.  Voxel s of
+ * channel c of global element e = elem_offset + b is kept iff its 32-bit
+ * number is at least ceil(p * 2^32).  The numbers of the 8 voxels of block
+ * q = c * ceil(H*W*D / 8) + s / 8 (s = (h * W + w) * D + d) are built from
+ * two Philox4x32-10 blocks of counter (q, e, e >> 32, STREAM | q >> 32) and
+ * key seed, STREAM = 0x44500000 for the high 16 bits and 0x44510000 for the
+ * low ones: half i (the low half of each word first) belongs to voxel
+ * 8 q' + i.  Channelwise: the number of channel c is that of lane c % 8 of
+ * block c / 8 of the streams 0x44520000 and 0x44530000.  A dropped value is
+ * +0 whatever it was; p outside [0, 1] is clamped, NaN counts as 0.  The
+ * backward pass is the same call on the gradient.  dst may equal src.
+ */
+typedef struct ba_dropout_desc {
+  const void* src; /* (B, C, H, W, D) in `layout` */
+  void* dst;       /* same shape, dtype and layout; may equal src, no partial overlap */
+  int64_t batch, channels, H, W, D;
+  int32_t dtype;   /* ba_dtype */
+  int32_t layout;  /* ba_layout */
+  int32_t flags;   /* BA_DROPOUT_* */
+  float p;         /* drop probability of every element, unless p_elem */
+  const float* p_elem;      /* (B,) or NULL: drop probabilities */
+  const uint8_t* mask;      /* (B,) 0/1 or NULL: elements with 0 are copied */
+  uint64_t seed;
+  const uint64_t* seed_dev; /* the seed in device memory, read when the kernel
+                               runs (a captured graph then draws other bits
+                               when the caller changes it), or NULL */
+  uint64_t elem_offset;     /* global index of element 0 */
+} ba_dropout_desc;
+BA_API ba_status ba_dropout(const ba_dropout_desc* desc, ba_stream_t stream);
+
+/*
+ * Group norm over groups of channels / groups consecutive channels and all
+ * voxels of an element, an optional per-channel affine, an activation, and a
+ * dropout (as ba_dropout, voxelwise, rescaled) of the result:
+ *   z = (x - mean) / sqrt(var + eps) * weight + bias  (var: biased),
+ *   out = dropout(activation(z)).
+ * Statistics and arithmetic in fp32 or more, one rounding at the store.
+ * ba_norm_forward reads x and writes out = y and stats; ba_norm_backward
+ * reads x, stats and dy (the gradient of y) and writes out = dx and, where
+ * given, dweight and dbias (dy and dx in x's dtype and layout).  Results do
+ * not depend on timing: no sum has an order of its own.  out overlaps neither
+ * x nor dy.
+ * workspace: ba_norm_workspace_bytes(desc, backward) bytes of device scratch,
+ * 16-byte aligned.
+ */
+typedef struct ba_norm_desc {
+  const void* x;  /* (B, C, H, W, D) in `layout` */
+  const void* dy; /* backward */
+  void* out;      /* y, or dx (backward: NULL when dx is not wanted) */
+  const void* weight; /* (C,) or NULL = ones */
+  const void* bias;   /* (C,) or NULL = zeros */
+  void* dweight;      /* backward: (C,) of param_dtype, or NULL */
+  void* dbias;
+  float* stats; /* (B, groups, 2): mean and 1 / sqrt(var + eps) */
+  int64_t batch, channels, H, W, D, groups;
+  int32_t dtype;       /* ba_dtype of x, dy, out */
+  int32_t layout;      /* ba_layout */
+  int32_t param_dtype; /* ba_dtype of weight, bias, dweight, dbias */
+  int32_t activation;  /* ba_activation */
+  float eps;           /* >= 0 */
+  float slope;         /* BA_ACT_LEAKY_RELU */
+  float p;             /* drop probability (0: no dropout), unless p_elem */
+  int32_t reserved;
+  const float* p_elem; /* (B,) or NULL */
+  uint64_t seed;
+  const uint64_t* seed_dev; /* see ba_dropout_desc */
+  uint64_t elem_offset;
+} ba_norm_desc;
+BA_API size_t ba_norm_workspace_bytes(const ba_norm_desc* desc, int32_t backward);
+BA_API ba_status ba_norm_forward(const ba_norm_desc* desc, void* workspace,
+                                 size_t workspace_bytes, ba_stream_t stream);
+BA_API ba_status ba_norm_backward(const ba_norm_desc* desc, void* workspace,
+                                  size_t workspace_bytes, ba_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
 /* Gaussian smoothing and the elastic field                                */
 /* ---------------------------------------------------------------------- */
 

@@ -1,0 +1,125 @@
+"""Group norm and dropout without a GPU: refusals of the C ABI and of the
+functions, scratch sizes, struct layouts."""
+from __future__ import annotations
+
+import ctypes
+import os
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import feature_ref as R
+from conftest import ROOT
+
+
+def _drop(L, **kw):
+    d = L.DropoutDesc(4096, 8192, 2, 3, 4, 4, 4, L.BA_F32, L.BA_CHANNELS_FIRST,
+                      L.BA_DROPOUT_RESCALE, 0.5)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _norm(L, **kw):
+    # made-up addresses: every call here is refused before a launch
+    d = L.NormDesc(x=1 << 20, dy=1 << 21, out=1 << 22, stats=1 << 23, batch=2, channels=6, H=4,
+                   W=4, D=4, groups=3, dtype=L.BA_F32, layout=L.BA_CHANNELS_LAST, eps=1e-5)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_struct_layouts_match_header(ba, tmp_path):
+    from batchaug_b200 import _lib as L
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    structs = {"ba_dropout_desc": L.DropoutDesc, "ba_norm_desc": L.NormDesc}
+    lines = ['#include <stdio.h>', '#include "batchaug_b200.h"', "int main(void) {"]
+    for cname, ct in structs.items():
+        lines.append(f'printf("{cname} size %zu\\n", sizeof({cname}));')
+        for fname, _ in ct._fields_:
+            lines.append(f'printf("{cname} {fname} %zu\\n", offsetof({cname}, {fname}));')
+    src = tmp_path / "probe.c"
+    src.write_text("\n".join(lines + ["return 0;", "}"]))
+    exe = tmp_path / "probe"
+    subprocess.run([cc, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split("\n")
+    lines = [line.split() for line in got if line]
+    assert len(lines) == sum(len(c._fields_) + 1 for c in structs.values())
+    for cname, what, val in lines:
+        ct = structs[cname]
+        assert int(val) == (ctypes.sizeof(ct) if what == "size" else getattr(ct, what).offset)
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(dtype=7), b"dtype"), (dict(layout=2), b"layout"), (dict(flags=8), b"flags"),
+    (dict(p=1.5), b"p="), (dict(p=float("nan")), b"p="), (dict(batch=-1), b"negative"),
+    (dict(src=None), b"NULL"), (dict(dst=None), b"NULL"), (dict(src=4098), b"aligned"),
+    (dict(dst=4096 + 64), b"overlaps"), (dict(p_elem=2), b"aligned"), (dict(seed_dev=4), b"aligned"),
+    (dict(H=1 << 30, W=1 << 30), b"2^40"), (dict(batch=1 << 31, channels=1, H=1, W=1, D=1), b"2^31"),
+])
+def test_dropout_refusals(ba, kw, word):
+    from batchaug_b200 import _lib as L
+    assert L.lib.ba_dropout(ctypes.byref(_drop(L, **kw)), None) == L.BA_EINVAL
+    assert word in L.lib.ba_last_error()
+    assert L.lib.ba_dropout(None, None) == L.BA_EINVAL
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(dtype=7), b"dtype"), (dict(layout=2), b"layout"), (dict(groups=0), b"groups"),
+    (dict(groups=4), b"divide"), (dict(param_dtype=3), b"param_dtype"),
+    (dict(activation=9), b"activation"), (dict(eps=-1.0), b"eps"), (dict(eps=float("nan")), b"eps"),
+    (dict(p=-0.5), b"p="), (dict(x=None), b"NULL"), (dict(stats=None), b"NULL"),
+    (dict(x=(1 << 20) + 2), b"aligned"), (dict(stats=(1 << 23) + 4), b"aligned"),
+    (dict(weight=2), b"aligned"), (dict(out=(1 << 20) + 16), b"overlaps"),
+    (dict(batch=1 << 30, channels=6, groups=6, H=1, W=1, D=1), b"2^31"),
+])
+@pytest.mark.parametrize("backward", [False, True])
+def test_norm_refusals(ba, kw, word, backward):
+    from batchaug_b200 import _lib as L
+    fn = L.lib.ba_norm_backward if backward else L.lib.ba_norm_forward
+    assert fn(ctypes.byref(_norm(L, **kw)), 1 << 24, 1 << 30, None) == L.BA_EINVAL
+    assert word in L.lib.ba_last_error()
+    assert fn(None, None, 0, None) == L.BA_EINVAL
+
+
+def test_norm_scratch_is_checked(ba):
+    from batchaug_b200 import _lib as L
+    d = _norm(L)
+    for backward, fn in ((0, L.lib.ba_norm_forward), (1, L.lib.ba_norm_backward)):
+        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(d), backward)
+        assert size > 0
+        assert fn(ctypes.byref(d), 1 << 24, size - 1, None) == L.BA_EINVAL
+        assert b"workspace" in L.lib.ba_last_error()
+        assert fn(ctypes.byref(d), (1 << 24) + 8, size, None) == L.BA_EINVAL
+        assert b"aligned" in L.lib.ba_last_error()
+    assert L.lib.ba_norm_workspace_bytes(ctypes.byref(_norm(L, groups=4)), 0) == 0
+    assert L.lib.ba_norm_workspace_bytes(ctypes.byref(_norm(L, D=0)), 0) == 0
+    # the backward pass alone reads dy
+    d = _norm(L, dy=None)
+    assert L.lib.ba_norm_backward(ctypes.byref(d), 1 << 24, 1 << 30, None) == L.BA_EINVAL
+    # nothing to do
+    for fn in (L.lib.ba_norm_forward, L.lib.ba_norm_backward):
+        assert fn(ctypes.byref(_norm(L, batch=0, x=None, out=None)), None, 0, None) == L.BA_OK
+    assert L.lib.ba_dropout(ctypes.byref(_drop(L, W=0, src=None)), None) == L.BA_OK
+
+
+def test_functions_want_cuda_tensors(ba):
+    from batchaug_b200 import ops
+    x = torch.zeros(2, 4, 3, 3, 3)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.group_norm(x, 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.dropout(x, 0.5, 1)
+
+
+def test_reference_bits_known_answer():
+    """The tests' own generator against Random123's published vectors."""
+    w = R.philox(0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344, 0x299F31D0A4093822)
+    assert [int(v) for v in w] == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    r = R.numbers(2, 3, 1000, 5)
+    assert abs(r.mean() / 2**32 - 0.5) < 0.02 and len(np.unique(r)) == r.size
