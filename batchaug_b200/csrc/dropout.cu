@@ -13,34 +13,52 @@ struct DropoutArgs {
   int32_t channelwise;
 };
 
+// 8 rows of the thread's columns a pass, each channel's bits from one block.
 template <int DT, int VEC>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_last(const __grid_constant__ DropoutArgs a) {
-  const LastPlace p = last_place<VEC>(a.f);
+  const int64_t b = blockIdx.x / a.f.nchunk;
+  const LastPlace p = last_place<VEC>(a.f, b, blockIdx.x - b * a.f.nchunk, blockIdx.y);
   if (!p.on) return;
   const DropRate dr = drop_rate(a.drop, p.b);
-  const int64_t base = p.b * a.f.S * a.f.C + p.c;
+  const int64_t base = last_base<DT>(a.f, p);
+  const char* src = (const char*)a.src + base;
+  char* dst = (char*)a.dst + base;
+  const uint32_t row = (uint32_t)a.f.C * ESIZE<DT>;
+  const F2 scale = f2(dr.scale);
   uint32_t keep[VEC];
   if (a.channelwise) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) keep[i] = drop_keep_channel(dr, p.c + i) ? 0xFFu : 0u;
+    for (int i = 0; i < VEC; ++i) keep[i] = drop_keep_channel(dr, p.c + i) ? KEEP_ALL : 0u;
   }
-  for (int64_t r = p.r0 + p.ty * 8; r < p.r1; r += p.nty * 8) {
-    Raw<DT, VEC> rx[8];
-    const int n = (int)min((int64_t)8, p.r1 - r);
+  for (int r = p.ty * 8; r < p.rows; r += p.nty * 8) {
+    Raw<DT, VEC> x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) rx[j] = raw_load<DT, VEC>(a.src, base + (r + j) * a.f.C);
-    if (!a.channelwise) last_keep<VEC>(a.f, dr, p.c, r, keep);
+      if (r + j < p.rows) x[j] = raw_load<DT, VEC>(src + row_at(r + j, row));
+    if (!a.channelwise) last_keep<VEC>(a.f, dr, p, r, keep);
+    if constexpr (VEC > 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) {
-        float v[VEC];
-        raw_unpack<DT, VEC>(rx[j], v);
+      for (int j = 0; j < 8; ++j) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = (keep[i] >> j) & 1u ? v[i] * dr.scale : 0.0f;
-        raw_store<DT, VEC>(a.dst, base + (r + j) * a.f.C, raw_pack<DT, VEC>(v));
+        for (int i = 0; i < VEC / 2; ++i)
+          raw_set_pair<DT, VEC>(
+              x[j], i,
+              last_pair_keep<DT>(
+                  pair_raw<DT>(mul2(pair_value<DT>(raw_pair<DT, VEC>(x[j], i)), scale)), keep, i,
+                  j));
+        if (r + j < p.rows) raw_store<DT, VEC>(dst + row_at(r + j, row), x[j]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const uint32_t k = keep[0] << (j >> 1);
+        const RawPair<DT> y = pair_keep<DT, 1, 3>(
+            pair_raw<DT>(mul2(pair_value<DT>(raw_join<DT>(x[j], x[j + 1])), scale)), k, k);
+        if (r + j < p.rows) raw_store<DT, 1>(dst + row_at(r + j, row), raw_half<DT>(y, 0));
+        if (r + j + 1 < p.rows) raw_store<DT, 1>(dst + row_at(r + j + 1, row), raw_half<DT>(y, 1));
+      }
+    }
   }
 }
 
@@ -48,28 +66,34 @@ template <int DT, int VEC>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_first(const __grid_constant__ DropoutArgs a) {
   FirstPlace p;
-  if (!first_place(a.f, p)) return;
+  if (!first_place(a.f, (int64_t)blockIdx.x * FEAT_WARPS + threadIdx.x / 32, p)) return;
   const DropRate dr = drop_rate(a.drop, p.b);
   constexpr int FLIGHT = 4;
-  const uint32_t row = a.channelwise ? (drop_keep_channel(dr, p.c) ? 0xFFu : 0u) : 0u;
-  for (int64_t s = p.s0; s < p.s1; s += FEAT_TILE * FLIGHT) {
-    FirstTile<DT, VEC> t[FLIGHT];
+  const char* src = (const char*)a.src + p.base * ESIZE<DT>;
+  char* dst = (char*)a.dst + p.base * ESIZE<DT>;
+  const F2 scale = f2(dr.scale);
+  uint32_t row = 0u;
+  if (a.channelwise) row = drop_keep_channel(dr, p.c) ? 0xFFFFFFFFu : 0u;
+  for (int s = 0; s < p.n; s += FEAT_TILE * FLIGHT) {
+    FirstTile<DT> t[FLIGHT];
 #pragma unroll
-    for (int u = 0; u < FLIGHT; ++u) first_load<DT, VEC>(a.src, p, s + u * FEAT_TILE, t[u]);
+    for (int u = 0; u < FLIGHT; ++u) first_load<DT, VEC>(src, s + u * FEAT_TILE, p, t[u]);
 #pragma unroll
     for (int u = 0; u < FLIGHT; ++u) {
-      const int64_t su = s + u * FEAT_TILE;
-      if (su < p.s1) {
-        const uint32_t keep = a.channelwise ? row : first_keep<VEC>(a.f, dr, p, su);
-        float v[8];
-        first_unpack<DT, VEC>(t[u], v);
+      const int su = s + u * FEAT_TILE;
+      if (su < p.n) {
+        uint32_t keep[8 / VEC];
+        if (a.channelwise) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (keep >> i) & 1u ? v[i] * dr.scale : 0.0f;
+          for (int i = 0; i < 8 / VEC; ++i) keep[i] = row;
+        } else {
+          first_keep<VEC>(a.f, dr, p, su, keep);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; j += VEC)
-          if (su + first_at<VEC>(p.lane, j) < p.s1)
-            raw_store<DT, VEC>(a.dst, p.base + su + first_at<VEC>(p.lane, j),
-                               raw_pack<DT, VEC>(v + j));
+        for (int i = 0; i < 4; ++i)
+          t[u].p[i] = first_pair_keep<DT, VEC>(
+              pair_raw<DT>(mul2(pair_value<DT>(t[u].p[i]), scale)), keep, i);
+        first_store<DT, VEC>(dst, su, p, t[u]);
       }
     }
   }

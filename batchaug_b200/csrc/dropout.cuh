@@ -77,47 +77,57 @@ __device__ __forceinline__ U4 drop_block(const DropRate& r, uint64_t q, uint32_t
   return philox4x32_10(ctr, r.k0, r.k1);
 }
 
-// Bit i set: number i of block q stays.
-__device__ __forceinline__ uint32_t drop_keep8(const DropRate& r, uint64_t q,
-                                               uint32_t stream = STREAM_DROP,
-                                               uint32_t stream_low = STREAM_DROP_LOW) {
-  if (r.hi == 0u && r.lo == 0u) return 0xFFu;
+// The decisions of a block as a word K: number 2 j's is bit 15 - j, number
+// 2 j + 1's bit 31 - j (set: it stays), so that K << j has the pair's in the
+// sign bits of its halves, where one byte permutation spreads them into masks.
+constexpr uint32_t KEEP_ALL = 0xF000F000u;
+
+// Sign bits of the halves: a >= t, for two 16-bit values each.
+__device__ __forceinline__ uint32_t ge_halves(uint32_t a, uint32_t t) {
+  const uint32_t h = 0x80008000u;
+  const uint32_t d = (a | h) - (t & ~h);  // sign: the low 15 bits of a reach t's
+  return (a & ~t) | (~(a ^ t) & d);
+}
+
+static __device__ __noinline__ uint32_t drop_ties(const DropRate& r, uint64_t q, uint32_t stream_low,
+                                           const uint32_t* w, uint32_t keep) {
+  const U4 l = drop_block(r, q, stream_low);
+  const uint32_t v[4] = {l.x, l.y, l.z, l.w};
+  for (int j = 0; j < 4; ++j) {
+    if ((w[j] & 0xFFFFu) == r.hi && (v[j] & 0xFFFFu) < r.lo) keep &= ~(1u << (15 - j));
+    if ((w[j] >> 16) == r.hi && (v[j] >> 16) < r.lo) keep &= ~(1u << (31 - j));
+  }
+  return keep;
+}
+
+__device__ __forceinline__ uint32_t drop_keep(const DropRate& r, uint64_t q,
+                                              uint32_t stream = STREAM_DROP,
+                                              uint32_t stream_low = STREAM_DROP_LOW) {
   if (r.hi > 0xFFFFu) return 0u;
   const U4 b = drop_block(r, q, stream);
   const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-  const uint32_t t = r.hi << 16;
-  uint32_t keep = 0u, tie = 0u;
+  const uint32_t t = r.hi * 0x10001u;
+  uint32_t keep = 0u;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    keep |= (w[j] << 16 >= t ? 1u : 0u) << (2 * j);
-    keep |= (w[j] >= t ? 1u : 0u) << (2 * j + 1);
-  }
+  for (int j = 0; j < 4; ++j) keep |= (ge_halves(w[j], t) & 0x80008000u) >> j;
   if (r.lo != 0u) {
+    // a zero half of w ^ t: a tie
+    uint32_t tie = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      tie |= ((w[j] & 0xFFFFu) == r.hi ? 1u : 0u) << (2 * j);
-      tie |= (w[j] >> 16 == r.hi ? 1u : 0u) << (2 * j + 1);
+      const uint32_t x = w[j] ^ t;
+      tie |= (x - 0x00010001u) & ~x;
     }
-    if (tie != 0u) {
-      const U4 l = drop_block(r, q, stream_low);
-      const uint32_t v[4] = {l.x, l.y, l.z, l.w};
-      uint32_t ge = 0u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ge |= ((v[j] & 0xFFFFu) >= r.lo ? 1u : 0u) << (2 * j);
-        ge |= (v[j] >> 16 >= r.lo ? 1u : 0u) << (2 * j + 1);
-      }
-      keep &= ~tie | ge;
-    }
+    if (tie & 0x80008000u) keep = drop_ties(r, q, stream_low, w, keep);
   }
   return keep;
 }
 
 // Whether channel c of the element stays (channelwise dropout).
 __device__ __forceinline__ bool drop_keep_channel(const DropRate& r, int64_t c) {
-  const uint32_t k =
-      drop_keep8(r, (uint64_t)c >> 3, STREAM_DROP_CHANNEL, STREAM_DROP_CHANNEL_LOW);
-  return (k >> (c & 7)) & 1u;
+  const uint32_t k = drop_keep(r, (uint64_t)c >> 3, STREAM_DROP_CHANNEL, STREAM_DROP_CHANNEL_LOW);
+  const int i = (int)(c & 7);
+  return (k >> ((i & 1 ? 31 : 15) - (i >> 1))) & 1u;
 }
 
 }  // namespace ba

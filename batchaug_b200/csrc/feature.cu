@@ -35,8 +35,9 @@ ba_status feat_check(const char* what, int64_t B, int64_t C, int64_t H, int64_t 
     n *= dims[i];
   }
   // the dropout blocks of an element are counted in 48 bits
-  BA_REQUIRE(B < ((int64_t)1 << 31) && C < ((int64_t)1 << 31),
-             "%s: batch or channels exceed 2^31 - 1", what);
+  BA_REQUIRE(B < ((int64_t)1 << 31), "%s: batch exceeds 2^31 - 1", what);
+  // a row's bytes are a 32-bit stride
+  BA_REQUIRE(C < ((int64_t)1 << 29), "%s: channels exceed 2^29 - 1", what);
   return BA_OK;
 }
 
@@ -54,6 +55,7 @@ Feat feat_plan(int64_t B, int64_t C, int64_t S, int32_t dtype, int32_t layout,
   f.nblk = (S + 7) / 8;
   f.colblocks = 1;
   f.ncw = 1;
+  f.width = C;
   const int esz = dtype == BA_BF16 ? 2 : 4;
   const bool last = layout == BA_CHANNELS_LAST;
   const int64_t inner = last ? C : S;
@@ -67,6 +69,7 @@ Feat feat_plan(int64_t B, int64_t C, int64_t S, int32_t dtype, int32_t layout,
   if (last) {
     const int64_t ncol = C / f.vec;
     f.ncw = (int32_t)std::min<int64_t>(ncol, FEAT_THREADS);
+    f.width = (int64_t)f.ncw * f.vec;
     f.colblocks = (ncol + f.ncw - 1) / f.ncw;
     // a pass of the CTA over 8 rows a thread, repeated while there are
     // several times as many chunks as SMs

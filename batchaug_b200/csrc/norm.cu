@@ -1,122 +1,128 @@
-// ba_norm_forward / ba_norm_backward: host side, and the kernels that merge
-// the per-channel partials of norm.cuh into statistics and coefficients.
+// ba_norm_forward / ba_norm_backward: checks, the schedule, the launch.
 #include <string.h>
+
+#include <algorithm>
 
 #include "norm_launch.cuh"
 
 namespace ba {
 namespace {
 
-// Values a partial of chunk k stands for.
-__device__ __forceinline__ int64_t chunk_count(const Feat& f, int64_t k) {
-  return min(f.rows, f.S - k * f.rows);
-}
-
-// Partial number i (0 .. Cg * nchunk) of group g of element b, its chunk in k.
-template <bool LAST>
-__device__ __forceinline__ float2 group_part(const NormArgs& a, int64_t b, int64_t g, int64_t i,
-                                             int64_t& k) {
-  if constexpr (LAST) {
-    k = i / a.Cg;
-    return a.part[(b * a.f.nchunk + k) * a.f.C + g * a.Cg + (i - k * a.Cg)];
-  } else {
-    k = i % a.f.nchunk;
-    return a.part[(b * a.f.C + g * a.Cg) * a.f.nchunk + i];
-  }
-}
-
-// One CTA per (element, group): mean and M2 of the group from its partials,
-// merged in double: mean = sum n_i mean_i / n, then
-// M2 = sum M2_i + n_i (mean_i - mean)^2.
-template <bool LAST>
-__global__ void __launch_bounds__(FEAT_THREADS)
-    norm_stats(const __grid_constant__ NormArgs a) {
-  __shared__ double tmp[FEAT_WARPS];
-  const int64_t b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
-  const int64_t n_parts = a.Cg * a.f.nchunk;
-  const double n = (double)a.Cg * (double)a.f.S;
-  double s = 0.0, m2 = 0.0;
-  int64_t k;
-  for (int64_t i = threadIdx.x; i < n_parts; i += FEAT_THREADS) {
-    const float2 q = group_part<LAST>(a, b, g, i, k);
-    s += (double)chunk_count(a.f, k) * (double)q.x;
-  }
-  const double mean = block_sum(s, tmp) / n;
-  for (int64_t i = threadIdx.x; i < n_parts; i += FEAT_THREADS) {
-    const float2 q = group_part<LAST>(a, b, g, i, k);
-    const double d = (double)q.x - mean;
-    m2 += (double)q.y + (double)chunk_count(a.f, k) * d * d;
-  }
-  m2 = block_sum(m2, tmp);
-  if (threadIdx.x == 0) {
-    a.stats[2 * blockIdx.x] = (float)mean;
-    a.stats[2 * blockIdx.x + 1] = (float)(1.0 / sqrt(m2 / n + (double)a.eps));
-  }
-}
-
-// One CTA per (element, group): each channel's sums (one warp a channel), and
-// the group's two coefficients.
-template <bool LAST>
-__global__ void __launch_bounds__(FEAT_THREADS)
-    norm_coefs(const __grid_constant__ NormArgs a) {
-  __shared__ double tmp[FEAT_WARPS];
-  const int64_t b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  double s1 = 0.0, s2 = 0.0;
-  for (int64_t j = warp; j < a.Cg; j += FEAT_WARPS) {
-    const int64_t c = g * a.Cg + j;
-    double p = 0.0, q = 0.0;
-    for (int64_t k = lane; k < a.f.nchunk; k += 32) {
-      const float2 t = LAST ? a.part[(b * a.f.nchunk + k) * a.f.C + c]
-                            : a.part[(b * a.f.C + c) * a.f.nchunk + k];
-      p += (double)t.x;
-      q += (double)t.y;
-    }
-    p = warp_sum(p);
-    q = warp_sum(q);
-    if (lane == 0) {
-      a.chan[b * a.f.C + c] = make_float2((float)p, (float)q);
-      const double w = (double)norm_param(a.weight, a.w_bf16, c, 1.0f);
-      s1 += w * p;
-      s2 += w * q;
-    }
-  }
-  s1 = block_sum(s1, tmp);
-  s2 = block_sum(s2, tmp);
-  if (threadIdx.x == 0) {
-    const double n = (double)a.Cg * (double)a.f.S;
-    const double r = (double)a.stats[2 * blockIdx.x + 1];
-    a.coef[blockIdx.x] = make_float2((float)(r * s1 / n), (float)(r * r * s2 / n));
-  }
-}
-
-// The gradients of weight and bias: a channel's sums over the batch.
-__global__ void norm_param_grads(const __grid_constant__ NormArgs a) {
-  const int64_t c = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (c >= a.f.C) return;
-  double db = 0.0, dw = 0.0;
-  for (int64_t b = 0; b < a.f.B; ++b) {
-    const float2 t = a.chan[b * a.f.C + c];
-    db += (double)t.x;
-    dw += (double)t.y;
-  }
-  const int dt = a.w_bf16 ? BA_BF16 : BA_F32;
-  if (a.dweight != nullptr) store_f(a.dweight, dt, c, (float)dw);
-  if (a.dbias != nullptr) store_f(a.dbias, dt, c, (float)db);
-}
-
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+// Bytes of input that a wave's units hold together.  Half of L2's 126 MB
+// would fit twice with the output's lines beside it; the measured figures are
+// at norm_schedule.
+constexpr int64_t NORM_WAVE_BYTES = (int64_t)24 << 20;
+constexpr int64_t NORM_AHEAD_BYTES = (int64_t)64 << 20;
+constexpr int NORM_MAX_SMEM = 227 << 10;
+
+// The kernel of a call, and how many of its CTAs the device holds at once.
+NormKernel norm_kernel_of(const NormKind& k, int32_t dtype, int32_t layout) {
+  const bool last = layout == BA_CHANNELS_LAST;
+  return dtype == BA_BF16 ? (last ? norm_kernel_bf16_last(k) : norm_kernel_bf16_first(k))
+                          : (last ? norm_kernel_f32_last(k) : norm_kernel_f32_first(k));
+}
+
+// Shared memory of a CTA: norm_kernel's layout.
+size_t norm_smem(const NormArgs& a, bool last, int32_t dtype, bool backward) {
+  const Feat& f = a.f;
+  const size_t bytes = (size_t)f.vec * (dtype == BA_BF16 ? 2 : 4);
+  const size_t ring = f.vec == 1 ? 0 : FEAT_THREADS * bytes * 8 * (backward ? 2 : 1);
+  size_t n = FEAT_THREADS * sizeof(double2) +
+             (size_t)a.ugroups * (2 * sizeof(double2) + sizeof(GroupStat)) + ring;
+  if (last)
+    n += std::max((size_t)5 * f.ncw * f.vec, (size_t)2 * FEAT_THREADS * f.vec) * sizeof(float);
+  return n;
+}
+
+// CTAs of the kernel that an SM holds; also lifts its shared memory limit.
+int norm_occupancy(NormKernel fn, const NormKind& k, int32_t dtype, int32_t layout, size_t smem) {
+  // an idempotent cache: threads that fill an entry together write the same
+  static int cached[64][2][2][3][4][2][2];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  int& c = cached[dev][dtype][layout][k.vec == 1 ? 0 : k.vec == 4 ? 1 : 2][k.act][k.drop]
+                 [k.backward];
+  if (c == 0) {
+    cudaFuncAttributes at;
+    int regs = 0;
+    if (cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             NORM_MAX_SMEM) != cudaSuccess ||
+        cudaFuncGetAttributes(&at, (const void*)fn) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&regs, fn, FEAT_THREADS, 0) != cudaSuccess ||
+        regs < 1) {
+      cudaGetLastError();
+      return 1;
+    }
+    c = regs;
+  }
+  // 227 KB a CTA at most and 228 KB an SM, 1 KB of it a CTA's own
+  return std::min<int>(c, std::max<int>(1, (int)(((size_t)228 << 10) / (smem + 1024))));
+}
+
+// Column blocks (channels last): whole groups, whole columns, and at least 128
+// bytes of a row, so that a block's accesses fill their lines.
+void norm_columns(NormArgs& a, int32_t dtype) {
+  Feat& f = a.f;
+  // the least run of channels that is both
+  int64_t x = a.Cg, y = f.vec;
+  while (y != 0) {
+    const int64_t t = x % y;
+    x = y;
+    y = t;
+  }
+  const int64_t least = a.Cg / x * f.vec, line = 128 / (dtype == BA_BF16 ? 2 : 4);
+  // blocks of m such runs, m a divisor of their number, one to four lines
+  // wide if there is such an m; otherwise one block, unless it has so many
+  // groups that their sums would fill the shared memory
+  const int64_t runs = f.C / least, want = (line + least - 1) / least;
+  int64_t m = want;
+  while (m < runs && m <= 4 * want && runs % m != 0) ++m;
+  if (m > 4 * want && m < runs) m = f.C / a.Cg <= 1024 ? runs : 1;
+  m = std::min(m, runs);
+  f.width = m * least;
+  f.colblocks = runs / m;
+  f.ncw = (int32_t)std::min<int64_t>(f.width / f.vec, FEAT_THREADS);
+  a.ugroups = (int32_t)(f.width / a.Cg);
+}
+
+// Cuts the work for `ctas` resident CTAs: waves of units, items of a unit.
+void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ctas) {
+  Feat& f = a.f;
+  const bool last = d.layout == BA_CHANNELS_LAST;
+  a.units = last ? f.B * f.colblocks : f.B * a.G;
+  const int64_t unit_bytes = f.S * (last ? f.width : a.Cg) * (d.dtype == BA_BF16 ? 2 : 4) *
+                             (backward ? 2 : 1);
+  int64_t wave = std::min(a.units, std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes));
+  const int64_t waves = (a.units + wave - 1) / wave;
+  wave = (a.units + waves - 1) / waves;
+  a.wave = wave;
+  a.ahead = waves > 1 && 2 * wave * unit_bytes <= NORM_AHEAD_BYTES;
+  a.reverse = !a.ahead;
+  // parts of a channel's voxels, so that a wave has one item for each CTA
+  const int64_t grain = last ? 8 : FEAT_TILE;  // voxels: whole dropout blocks, whole tiles
+  const int64_t rows_of_unit = last ? 1 : a.Cg;
+  const int64_t workers = last ? ctas : ctas * FEAT_WARPS;
+  const int64_t least = last ? (int64_t)(FEAT_THREADS / f.ncw) * 8 : FEAT_TILE;
+  int64_t parts = std::max<int64_t>(1, workers / (wave * rows_of_unit));
+  parts = std::min(parts, (f.S + least - 1) / least);
+  f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
+  f.nchunk = (f.S + f.rows - 1) / f.rows;
+  a.items = (int32_t)(last ? f.nchunk : (a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
+}
+
 struct NormScratch {
-  size_t part, coef, chan, total;  // byte offsets
+  size_t sync, part, chan, total;  // byte offsets
 };
 
-NormScratch norm_scratch(const Feat& f, int64_t G, bool backward) {
+NormScratch norm_scratch(const NormArgs& a, bool backward) {
   NormScratch s;
-  s.part = 0;
-  s.coef = align16((size_t)(f.B * f.C * f.nchunk) * sizeof(float2));
-  s.chan = s.coef + (backward ? align16((size_t)(f.B * G) * sizeof(float2)) : 0);
-  s.total = s.chan + (backward ? align16((size_t)(f.B * f.C) * sizeof(float2)) : 0);
+  s.sync = 0;
+  s.part = align16((size_t)(1 + a.units) * sizeof(uint32_t));
+  s.chan = s.part + (size_t)(a.units * a.items * a.ugroups) * sizeof(float4);
+  s.total = s.chan +
+            (backward ? align16((size_t)(a.f.B * a.f.C * a.f.nchunk) * sizeof(float2)) : 0);
   return s;
 }
 
@@ -138,10 +144,42 @@ ba_status norm_check(const char* what, const ba_norm_desc* d) {
   return BA_OK;
 }
 
-Feat norm_plan(const ba_norm_desc& d, bool backward) {
+// Everything of a call that its sizes, types and addresses decide.
+struct NormCall {
+  NormArgs a;
+  NormKernel fn;
+  NormScratch scratch;
+  size_t smem;
+  int64_t ctas;
+};
+
+void norm_plan(const ba_norm_desc& d, bool backward, NormCall& c) {
+  NormArgs& a = c.a;
+  memset(&a, 0, sizeof(a));
   const void* ptrs[3] = {d.x, d.out, d.dy};
-  return feat_plan(d.batch, d.channels, d.H * d.W * d.D, d.dtype, d.layout, ptrs,
-                   backward ? 3 : 2);
+  a.f = feat_plan(d.batch, d.channels, d.H * d.W * d.D, d.dtype, d.layout, ptrs,
+                  backward ? 3 : 2);
+  a.G = d.groups;
+  a.Cg = d.channels / d.groups;
+  NormKind k;
+  k.vec = a.f.vec;
+  k.act = d.activation == BA_ACT_NONE   ? ACT_NONE
+          : d.activation == BA_ACT_SILU ? ACT_SILU
+          : d.activation == BA_ACT_GELU ? ACT_GELU
+                                        : ACT_LEAKY;
+  k.drop = d.p_elem != nullptr || d.p > 0.0f;
+  k.backward = backward;
+  c.fn = norm_kernel_of(k, d.dtype, d.layout);
+  const bool last = d.layout == BA_CHANNELS_LAST;
+  if (last)
+    norm_columns(a, d.dtype);
+  else
+    a.ugroups = 1;
+  c.smem = norm_smem(a, last, d.dtype, backward);
+  c.ctas = (int64_t)norm_occupancy(c.fn, k, d.dtype, d.layout, c.smem) * device_sms();
+  norm_schedule(a, d, backward, c.ctas);
+  c.scratch = norm_scratch(a, backward);
+  a.inv_n = 1.0 / ((double)a.Cg * (double)a.f.S);
 }
 
 ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, void* workspace,
@@ -173,10 +211,18 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   BA_REQUIRE(d.out == nullptr || (!feat_overlap(d.x, d.out, bytes) &&
                                   (!backward || !feat_overlap(d.dy, d.out, bytes))),
              "%s: out overlaps an input", what);
-  NormArgs a;
-  memset(&a, 0, sizeof(a));
-  a.f = norm_plan(d, backward);
-  const NormScratch sc = norm_scratch(a.f, d.groups, backward);
+  NormCall c;
+  norm_plan(d, backward, c);
+  NormArgs& a = c.a;
+  const NormScratch& sc = c.scratch;
+  // counts are 32 bits: an item's rows, a partial's values, the items of a launch
+  const double part_values =
+      (double)a.f.rows * (double)(d.layout == BA_CHANNELS_LAST ? a.Cg : (int64_t)FEAT_WARPS);
+  if (a.f.rows >= ((int64_t)1 << 31) || part_values >= 4294967296.0 ||
+      (double)a.units * (double)a.items >= 4294967296.0 || c.smem > (size_t)NORM_MAX_SMEM) {
+    set_error("%s: tensor too large for one launch", what);
+    return BA_EUNSUPPORTED;
+  }
   BA_REQUIRE(workspace != nullptr && workspace_bytes >= sc.total,
              "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0,
              sc.total);
@@ -190,53 +236,23 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.dbias = d.dbias;
   a.w_bf16 = d.param_dtype == BA_BF16;
   a.stats = d.stats;
-  a.part = (float2*)((char*)workspace + sc.part);
-  a.coef = (float2*)((char*)workspace + sc.coef);
-  a.chan = (float2*)((char*)workspace + sc.chan);
-  a.G = d.groups;
-  a.Cg = d.channels / d.groups;
+  a.sync = (uint32_t*)((char*)workspace + sc.sync);
+  a.part = (float4*)((char*)workspace + sc.part);
+  a.chan = d.dweight || d.dbias ? (float2*)((char*)workspace + sc.chan) : nullptr;
+  a.timeouts = wait_timeouts(cs);
   a.eps = d.eps;
   a.slope = d.activation == BA_ACT_LEAKY_RELU ? d.slope : 0.0f;
   a.drop = {d.p, d.p_elem, nullptr, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
             d.elem_offset, 1};
-  const bool last = d.layout == BA_CHANNELS_LAST;
-  NormLaunch l;
-  l.act = d.activation == BA_ACT_NONE   ? ACT_NONE
-          : d.activation == BA_ACT_SILU ? ACT_SILU
-          : d.activation == BA_ACT_GELU ? ACT_GELU
-                                        : ACT_LEAKY;
-  l.drop = d.p_elem != nullptr || d.p > 0.0f;
-  l.stream = cs;
-  st = feat_grid(what, a.f, d.layout, &l.grid);
-  if (st != BA_OK) return st;
-  auto launch = [&](int step) {
-    l.step = step;
-    if (d.dtype == BA_BF16)
-      last ? norm_launch_bf16_last(a, l) : norm_launch_bf16_first(a, l);
-    else
-      last ? norm_launch_f32_last(a, l) : norm_launch_f32_first(a, l);
-    return check_launch(what);
-  };
-  const unsigned groups = (unsigned)(d.batch * d.groups);
-  if ((st = launch(backward ? NORM_BWD_SUMS : NORM_SUMS)) != BA_OK) return st;
-  if (!backward) {
-    if (last)
-      norm_stats<true><<<groups, FEAT_THREADS, 0, cs>>>(a);
-    else
-      norm_stats<false><<<groups, FEAT_THREADS, 0, cs>>>(a);
-    if ((st = check_launch(what)) != BA_OK) return st;
-    return launch(NORM_APPLY);
+  if (cudaMemsetAsync(a.sync, 0, sc.part, cs) != cudaSuccess) {
+    set_error("%s: clearing the scratch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return BA_ECUDA;
   }
-  if (last)
-    norm_coefs<true><<<groups, FEAT_THREADS, 0, cs>>>(a);
-  else
-    norm_coefs<false><<<groups, FEAT_THREADS, 0, cs>>>(a);
-  if ((st = check_launch(what)) != BA_OK) return st;
-  if (a.dweight != nullptr || a.dbias != nullptr) {
-    norm_param_grads<<<(unsigned)((d.channels + 255) / 256), 256, 0, cs>>>(a);
-    if ((st = check_launch(what)) != BA_OK) return st;
-  }
-  return d.out != nullptr ? launch(NORM_BWD_APPLY) : BA_OK;
+  const unsigned grid = (unsigned)std::min(c.ctas, a.wave * a.items);
+  void* args[1] = {&a};
+  cudaLaunchCooperativeKernel((const void*)c.fn, dim3(grid), dim3(FEAT_THREADS), args,
+                              c.smem, cs);
+  return check_launch(what);
 }
 
 }  // namespace
@@ -247,7 +263,9 @@ extern "C" size_t ba_norm_workspace_bytes(const ba_norm_desc* desc, int32_t back
   clear_error();
   if (norm_check("ba_norm_workspace_bytes", desc) != BA_OK) return 0;
   if (desc->batch * desc->channels * desc->H * desc->W * desc->D == 0) return 0;
-  return norm_scratch(norm_plan(*desc, backward != 0), desc->groups, backward != 0).total;
+  NormCall c;
+  norm_plan(*desc, backward != 0, c);
+  return c.scratch.total;
 }
 
 extern "C" ba_status ba_norm_forward(const ba_norm_desc* desc, void* workspace,

@@ -1,9 +1,7 @@
 // norm.cuh for bf16 tensors, channels first.
 #include "norm_launch.cuh"
 
-void ba::norm_launch_bf16_first(const NormArgs& a, const NormLaunch& l) {
-  if (a.f.vec == 8)
-    norm_launch_vec<BA_BF16, false, 8>(a, l);
-  else
-    norm_launch_vec<BA_BF16, false, 1>(a, l);
+ba::NormKernel ba::norm_kernel_bf16_first(const NormKind& k) {
+  if (k.vec == 8) return norm_kernel_vec<BA_BF16, false, 8>(k);
+  return norm_kernel_vec<BA_BF16, false, 1>(k);
 }

@@ -1,11 +1,8 @@
 // norm.cuh for bf16 tensors, channels last.
 #include "norm_launch.cuh"
 
-void ba::norm_launch_bf16_last(const NormArgs& a, const NormLaunch& l) {
-  if (a.f.vec == 8)
-    norm_launch_vec<BA_BF16, true, 8>(a, l);
-  else if (a.f.vec == 4)
-    norm_launch_vec<BA_BF16, true, 4>(a, l);
-  else
-    norm_launch_vec<BA_BF16, true, 1>(a, l);
+ba::NormKernel ba::norm_kernel_bf16_last(const NormKind& k) {
+  if (k.vec == 8) return norm_kernel_vec<BA_BF16, true, 8>(k);
+  if (k.vec == 4) return norm_kernel_vec<BA_BF16, true, 4>(k);
+  return norm_kernel_vec<BA_BF16, true, 1>(k);
 }

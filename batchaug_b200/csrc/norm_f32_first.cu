@@ -1,9 +1,7 @@
 // norm.cuh for fp32 tensors, channels first.
 #include "norm_launch.cuh"
 
-void ba::norm_launch_f32_first(const NormArgs& a, const NormLaunch& l) {
-  if (a.f.vec == 4)
-    norm_launch_vec<BA_F32, false, 4>(a, l);
-  else
-    norm_launch_vec<BA_F32, false, 1>(a, l);
+ba::NormKernel ba::norm_kernel_f32_first(const NormKind& k) {
+  if (k.vec == 4) return norm_kernel_vec<BA_F32, false, 4>(k);
+  return norm_kernel_vec<BA_F32, false, 1>(k);
 }

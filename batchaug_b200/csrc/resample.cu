@@ -37,6 +37,7 @@
 #include <mutex>
 
 #include "ba_common.cuh"
+#include "feature.cuh"
 
 namespace ba {
 namespace {
@@ -1864,8 +1865,8 @@ constexpr int PT_STAGES = BA_PT_STAGES;
 constexpr int PT_MAX_DIM = 256;  // tensor-map box extent limit; also the tables
 constexpr unsigned long long PT_WAIT_NS = 2000000000ull;
 
-// Bounded device waits that ran out (any kernel of this file); read and
-// cleared by ba_wait_status.
+// Bounded device waits that ran out (kernels of this file, and those given its
+// address by wait_timeouts); read and cleared by ba_wait_status.
 __device__ unsigned int g_wait_timeouts;
 
 struct PermTmaArgs {
@@ -3176,6 +3177,20 @@ extern "C" ba_status ba_compose_field(const float* field, const float* theta,
   compose_field_kernel<<<g, 256, 0, (cudaStream_t)stream>>>(field, theta, mask_field, mask_affine,
                                                           (int)H, (int)W, (int)D, grid);
   return check_launch("ba_compose_field");
+}
+
+unsigned int* ba::wait_timeouts(cudaStream_t stream) {
+  static unsigned int* cached[64] = {nullptr};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (cached[dev] == nullptr) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone)
+      return nullptr;
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_wait_timeouts) == cudaSuccess) cached[dev] = (unsigned int*)p;
+  }
+  return cached[dev];
 }
 
 extern "C" ba_status ba_wait_status(ba_stream_t stream) {
