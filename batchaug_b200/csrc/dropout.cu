@@ -17,7 +17,7 @@ struct DropoutArgs {
 template <int DT, int VEC>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_last(const __grid_constant__ DropoutArgs a) {
-  const int64_t b = blockIdx.x / a.f.nchunk;
+  const uint32_t b = blockIdx.x / a.f.nchunk;
   const LastPlace p = last_place<VEC>(a.f, b, blockIdx.x - b * a.f.nchunk, blockIdx.y);
   if (!p.on) return;
   const DropRate dr = drop_rate(a.drop, p.b);
@@ -66,7 +66,7 @@ template <int DT, int VEC>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_first(const __grid_constant__ DropoutArgs a) {
   FirstPlace p;
-  if (!first_place(a.f, (int64_t)blockIdx.x * FEAT_WARPS + threadIdx.x / 32, p)) return;
+  if (!first_place(a.f, blockIdx.x * FEAT_WARPS + threadIdx.x / 32, p)) return;
   const DropRate dr = drop_rate(a.drop, p.b);
   constexpr int FLIGHT = 4;
   const char* src = (const char*)a.src + p.base * ESIZE<DT>;

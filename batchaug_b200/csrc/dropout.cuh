@@ -73,8 +73,20 @@ __device__ __forceinline__ DropRate drop_rate(const DropArgs& a, int64_t b) {
 }
 
 __device__ __forceinline__ U4 drop_block(const DropRate& r, uint64_t q, uint32_t stream) {
-  const U4 ctr = {(uint32_t)q, r.e_lo, r.e_hi, stream | (uint32_t)(q >> 32)};
-  return philox4x32_10(ctr, r.k0, r.k1);
+  // philox4x32_10 with each 64-bit product as one instruction
+  uint32_t x = (uint32_t)q, y = r.e_lo, z = r.e_hi, w = stream | (uint32_t)(q >> 32);
+  uint32_t k0 = r.k0, k1 = r.k1;
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)0xD2511F53u * x, b = (uint64_t)0xCD9E8D57u * z;
+    x = (uint32_t)(b >> 32) ^ y ^ k0;
+    y = (uint32_t)b;
+    z = (uint32_t)(a >> 32) ^ w ^ k1;
+    w = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return {x, y, z, w};
 }
 
 // The decisions of a block as a word K: number 2 j's is bit 15 - j, number

@@ -70,7 +70,7 @@ Feat feat_plan(int64_t B, int64_t C, int64_t S, int32_t dtype, int32_t layout,
     const int64_t ncol = C / f.vec;
     f.ncw = (int32_t)std::min<int64_t>(ncol, FEAT_THREADS);
     f.width = (int64_t)f.ncw * f.vec;
-    f.colblocks = (ncol + f.ncw - 1) / f.ncw;
+    f.colblocks = (uint32_t)((ncol + f.ncw - 1) / f.ncw);
     // a pass of the CTA over 8 rows a thread, repeated while there are
     // several times as many chunks as SMs
     const int64_t unit = (int64_t)(FEAT_THREADS / f.ncw) * 8;
@@ -80,16 +80,16 @@ Feat feat_plan(int64_t B, int64_t C, int64_t S, int32_t dtype, int32_t layout,
   } else {
     f.rows = (int64_t)FEAT_TILE * FEAT_RUN;
   }
-  f.nchunk = (S + f.rows - 1) / f.rows;
+  f.nchunk = (uint32_t)((S + f.rows - 1) / f.rows);
   return f;
 }
 
 ba_status feat_grid(const char* what, const Feat& f, int32_t layout, dim3* grid) {
-  const int64_t x = layout == BA_CHANNELS_LAST
-                        ? f.B * f.nchunk
-                        : (f.B * f.C * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS;
+  const int64_t items = f.B * (layout == BA_CHANNELS_LAST ? 1 : f.C) * (int64_t)f.nchunk;
+  const int64_t x =
+      layout == BA_CHANNELS_LAST ? items : (items + FEAT_WARPS - 1) / FEAT_WARPS;
   const int64_t y = layout == BA_CHANNELS_LAST ? f.colblocks : 1;
-  if (x > 0x7FFFFFFF || y > 65535) {
+  if (x > 0x7FFFFFFF || y > 65535 || items > 0xFFFFFFFF - FEAT_WARPS) {
     set_error("%s: tensor too large for one launch", what);
     return BA_EUNSUPPORTED;
   }

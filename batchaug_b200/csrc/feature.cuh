@@ -20,8 +20,10 @@ struct Feat {
   int64_t B, C, S;
   int64_t nblk;       // ceil(S / 8): dropout blocks of a channel
   int64_t rows;       // voxels of a chunk, below 2^31
-  int64_t nchunk;     // chunks of a channel
-  int64_t colblocks;  // channels-last: column blocks, of `width` channels
+  // counts that index divisions use are 32 bits (a 64-bit division is a call
+  // of a hundred instructions, as many as a thread spends on ten accesses)
+  uint32_t nchunk;    // chunks of a channel
+  uint32_t colblocks; // channels-last: column blocks, of `width` channels
   int64_t width;
   int32_t ncw;        // channels-last: threads of a row (columns of VEC channels)
   int32_t vec;        // elements of a memory access
@@ -47,36 +49,34 @@ ba_status feat_grid(const char* what, const Feat& f, int32_t layout, dim3* grid)
 // (one issue slot for two results, each rounded as the scalar operation).
 // ---------------------------------------------------------------------------
 struct F2 {
-  float x, y;
+  unsigned long long v;  // kept whole, so that the pair stays in place
+  __device__ __forceinline__ float x() const {
+    return __uint_as_float((uint32_t)v);
+  }
+  __device__ __forceinline__ float y() const {
+    return __uint_as_float((uint32_t)(v >> 32));
+  }
 };
-__device__ __forceinline__ F2 f2(float x, float y) { return {x, y}; }
-__device__ __forceinline__ F2 f2(float x) { return {x, x}; }
-__device__ __forceinline__ unsigned long long f2_bits(F2 a) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
   return r;
 }
-__device__ __forceinline__ F2 f2_from(unsigned long long r) {
-  F2 a;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
-  return a;
-}
+__device__ __forceinline__ F2 f2(float x) { return f2(x, x); }
 __device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_from(r);
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_from(r);
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
-  return f2_from(r);
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
 }
 
 // ---------------------------------------------------------------------------
@@ -113,9 +113,9 @@ __device__ __forceinline__ F2 pair_value(RawPair<DT> p) {
 template <int DT>
 __device__ __forceinline__ RawPair<DT> pair_raw(F2 v) {
   if constexpr (DT == BA_BF16)
-    return pack_bf16x2(v.x, v.y);
+    return pack_bf16x2(v.x(), v.y());
   else
-    return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
+    return make_uint2(__float_as_uint(v.x()), __float_as_uint(v.y()));
 }
 
 // Pair i of VEC >= 2 elements.
@@ -193,16 +193,16 @@ struct LastPlace {
 };
 
 template <int VEC>
-__device__ __forceinline__ LastPlace last_place(const Feat& f, int64_t b, int64_t k, int64_t cb) {
+__device__ __forceinline__ LastPlace last_place(const Feat& f, uint32_t b, uint32_t k, uint32_t cb) {
   LastPlace p;
   p.tx = threadIdx.x % f.ncw;
   p.ty = threadIdx.x / f.ncw;
   p.nty = FEAT_THREADS / f.ncw;
   p.b = b;
   p.k = k;
-  p.c = cb * f.width + p.tx * VEC;
-  p.c_end = min((cb + 1) * f.width, f.C);
-  p.r0 = k * f.rows;
+  p.c = (int64_t)cb * f.width + p.tx * VEC;
+  p.c_end = min(((int64_t)cb + 1) * f.width, f.C);
+  p.r0 = (int64_t)k * f.rows;
   p.rows = (int)min(f.rows, f.S - p.r0);
   p.on = p.ty < p.nty && p.c < p.c_end;
   return p;
@@ -352,16 +352,16 @@ __device__ __forceinline__ RawPair<DT> first_pair_keep(RawPair<DT> p, const uint
 }
 
 // A grid-wide list of runs (no units): run number `item`.
-__device__ __forceinline__ bool first_place(const Feat& f, int64_t item, FirstPlace& p) {
+__device__ __forceinline__ bool first_place(const Feat& f, uint32_t item, FirstPlace& p) {
   p.lane = threadIdx.x % 32;
-  const int64_t row = item / f.nchunk;
-  p.k = item - row * f.nchunk;
-  p.b = row / f.C;
-  p.c = row - p.b * f.C;
-  p.s0 = p.k * f.rows;
+  const uint32_t row = item / f.nchunk, k = item - row * f.nchunk, b = row / (uint32_t)f.C;
+  p.k = k;
+  p.b = b;
+  p.c = row - b * (uint32_t)f.C;
+  p.s0 = k * f.rows;
   p.n = (int)min(f.rows, f.S - p.s0);
   p.base = row * f.S + p.s0;
-  return row < f.B * f.C;
+  return b < f.B;
 }
 
 }  // namespace ba

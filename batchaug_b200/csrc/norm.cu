@@ -10,11 +10,14 @@ namespace {
 
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-// Bytes of input that a wave's units hold together.  Half of L2's 126 MB
-// would fit twice with the output's lines beside it; the measured figures are
-// at norm_schedule.
-constexpr int64_t NORM_WAVE_BYTES = (int64_t)24 << 20;
-constexpr int64_t NORM_AHEAD_BYTES = (int64_t)64 << 20;
+// Inputs of the sets' waves together.  L2 (126 MB, each of the two dies with
+// lines of its own) keeps about 32 MB of them from the sums to the results,
+// with the outputs' lines beside them: on 268 MB in units of 4 MB, the DRAM
+// reads of a forward pass were 269 MB with waves of 16 MB, 285 at 32 MB, 368 at
+// 48 MB and 451 at 64 MB.  But every wave waits once, and that costs more than
+// the reads: 182, 143, 148 and 139 us.
+constexpr int64_t NORM_WAVE_BYTES = (int64_t)72 << 20;
+constexpr int64_t NORM_L2_BYTES = (int64_t)36 << 20;
 constexpr int NORM_MAX_SMEM = 227 << 10;
 
 // The kernel of a call, and how many of its CTAs the device holds at once.
@@ -29,10 +32,11 @@ size_t norm_smem(const NormArgs& a, bool last, int32_t dtype, bool backward) {
   const Feat& f = a.f;
   const size_t bytes = (size_t)f.vec * (dtype == BA_BF16 ? 2 : 4);
   const size_t ring = f.vec == 1 ? 0 : FEAT_THREADS * bytes * 8 * (backward ? 2 : 1);
-  size_t n = FEAT_THREADS * sizeof(double2) +
+  const size_t cw = (size_t)f.ncw * f.vec;
+  size_t n = std::max<size_t>(FEAT_THREADS, cw) * sizeof(double2) +
              (size_t)a.ugroups * (2 * sizeof(double2) + sizeof(GroupStat)) + ring;
   if (last)
-    n += std::max((size_t)5 * f.ncw * f.vec, (size_t)2 * FEAT_THREADS * f.vec) * sizeof(float);
+    n += ((cw + 3) / 4 * 4 + std::max(5 * cw, (size_t)2 * FEAT_THREADS * f.vec)) * sizeof(float);
   return n;
 }
 
@@ -82,24 +86,31 @@ void norm_columns(NormArgs& a, int32_t dtype) {
   if (m > 4 * want && m < runs) m = f.C / a.Cg <= 1024 ? runs : 1;
   m = std::min(m, runs);
   f.width = m * least;
-  f.colblocks = runs / m;
+  f.colblocks = (uint32_t)(runs / m);
   f.ncw = (int32_t)std::min<int64_t>(f.width / f.vec, FEAT_THREADS);
-  a.ugroups = (int32_t)(f.width / a.Cg);
+  a.ugroups = (uint32_t)(f.width / a.Cg);
 }
 
 // Cuts the work for `ctas` resident CTAs: waves of units, items of a unit.
 void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ctas) {
   Feat& f = a.f;
   const bool last = d.layout == BA_CHANNELS_LAST;
-  a.units = last ? f.B * f.colblocks : f.B * a.G;
+  const int64_t units = last ? f.B * f.colblocks : f.B * a.G;
+  a.units = (uint32_t)units;
   const int64_t unit_bytes = f.S * (last ? f.width : a.Cg) * (d.dtype == BA_BF16 ? 2 : 4) *
                              (backward ? 2 : 1);
-  int64_t wave = std::min(a.units, std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes));
-  const int64_t waves = (a.units + wave - 1) / wave;
-  wave = (a.units + waves - 1) / waves;
-  a.wave = wave;
-  a.ahead = waves > 1 && 2 * wave * unit_bytes <= NORM_AHEAD_BYTES;
-  a.reverse = !a.ahead;
+  // two sets of CTAs, so that one streams while the other waits (units of
+  // 33 MB, forward: 41 us, 59 us with one set; four sets of smaller waves were
+  // no better)
+  const int64_t sets = std::min<int64_t>(units, std::min<int64_t>(2, ctas / device_sms()));
+  int64_t wave = std::min((units + sets - 1) / sets,
+                          std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes / sets));
+  const int64_t waves = (units + wave * sets - 1) / (wave * sets) * sets;
+  wave = (units + waves - 1) / waves;
+  a.sets = (uint32_t)sets;
+  a.wave = (uint32_t)wave;
+  a.reverse = sets * wave * unit_bytes > NORM_L2_BYTES;
+  ctas /= sets;
   // parts of a channel's voxels, so that a wave has one item for each CTA
   const int64_t grain = last ? 8 : FEAT_TILE;  // voxels: whole dropout blocks, whole tiles
   const int64_t rows_of_unit = last ? 1 : a.Cg;
@@ -108,19 +119,19 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   int64_t parts = std::max<int64_t>(1, workers / (wave * rows_of_unit));
   parts = std::min(parts, (f.S + least - 1) / least);
   f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
-  f.nchunk = (f.S + f.rows - 1) / f.rows;
-  a.items = (int32_t)(last ? f.nchunk : (a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
+  f.nchunk = (uint32_t)((f.S + f.rows - 1) / f.rows);
+  a.items = (uint32_t)(last ? f.nchunk : ((int64_t)a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
 }
 
 struct NormScratch {
-  size_t sync, part, chan, total;  // byte offsets
+  size_t done, part, chan, total;  // byte offsets; up to chan: zeroed
 };
 
 NormScratch norm_scratch(const NormArgs& a, bool backward) {
   NormScratch s;
-  s.sync = 0;
-  s.part = align16((size_t)(1 + a.units) * sizeof(uint32_t));
-  s.chan = s.part + (size_t)(a.units * a.items * a.ugroups) * sizeof(float4);
+  s.done = 0;
+  s.part = 16;
+  s.chan = s.part + (size_t)a.units * a.items * a.ugroups * sizeof(float4);
   s.total = s.chan +
             (backward ? align16((size_t)(a.f.B * a.f.C * a.f.nchunk) * sizeof(float2)) : 0);
   return s;
@@ -159,8 +170,8 @@ void norm_plan(const ba_norm_desc& d, bool backward, NormCall& c) {
   const void* ptrs[3] = {d.x, d.out, d.dy};
   a.f = feat_plan(d.batch, d.channels, d.H * d.W * d.D, d.dtype, d.layout, ptrs,
                   backward ? 3 : 2);
-  a.G = d.groups;
-  a.Cg = d.channels / d.groups;
+  a.G = (uint32_t)d.groups;
+  a.Cg = (uint32_t)(d.channels / d.groups);
   NormKind k;
   k.vec = a.f.vec;
   k.act = d.activation == BA_ACT_NONE   ? ACT_NONE
@@ -217,9 +228,10 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   const NormScratch& sc = c.scratch;
   // counts are 32 bits: an item's rows, a partial's values, the items of a launch
   const double part_values =
-      (double)a.f.rows * (double)(d.layout == BA_CHANNELS_LAST ? a.Cg : (int64_t)FEAT_WARPS);
+      (double)a.f.rows * (double)(d.layout == BA_CHANNELS_LAST ? a.Cg : (uint32_t)FEAT_WARPS);
   if (a.f.rows >= ((int64_t)1 << 31) || part_values >= 4294967296.0 ||
-      (double)a.units * (double)a.items >= 4294967296.0 || c.smem > (size_t)NORM_MAX_SMEM) {
+      (double)a.units * (double)a.items * FEAT_WARPS >= 4294967296.0 ||
+      (double)a.f.B * (double)a.f.nchunk >= 4294967296.0 || c.smem > (size_t)NORM_MAX_SMEM) {
     set_error("%s: tensor too large for one launch", what);
     return BA_EUNSUPPORTED;
   }
@@ -236,7 +248,7 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.dbias = d.dbias;
   a.w_bf16 = d.param_dtype == BA_BF16;
   a.stats = d.stats;
-  a.sync = (uint32_t*)((char*)workspace + sc.sync);
+  a.done = (uint32_t*)((char*)workspace + sc.done);
   a.part = (float4*)((char*)workspace + sc.part);
   a.chan = d.dweight || d.dbias ? (float2*)((char*)workspace + sc.chan) : nullptr;
   a.timeouts = wait_timeouts(cs);
@@ -244,11 +256,12 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.slope = d.activation == BA_ACT_LEAKY_RELU ? d.slope : 0.0f;
   a.drop = {d.p, d.p_elem, nullptr, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
             d.elem_offset, 1};
-  if (cudaMemsetAsync(a.sync, 0, sc.part, cs) != cudaSuccess) {
+  if (cudaMemsetAsync(workspace, 0, sc.chan, cs) != cudaSuccess) {
     set_error("%s: clearing the scratch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
     return BA_ECUDA;
   }
-  const unsigned grid = (unsigned)std::min(c.ctas, a.wave * a.items);
+  const unsigned grid =
+      (unsigned)(a.sets * std::min<int64_t>(c.ctas / a.sets, (int64_t)a.wave * a.items));
   void* args[1] = {&a};
   cudaLaunchCooperativeKernel((const void*)c.fn, dim3(grid), dim3(FEAT_THREADS), args,
                               c.smem, cs);

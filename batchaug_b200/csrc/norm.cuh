@@ -11,18 +11,21 @@
 //
 // One cooperative launch does it all.  A unit is what is normalised on its
 // own: a group of an element (channels first), or the groups of a block of
-// columns of an element (channels last).  Units are taken in waves; the
-// resident CTAs share a wave's items (equal parts of its units' voxels), first
-// for the sums, then for the results.  Every CTA leaves a partial for each
-// group of its item and counts it; a CTA that needs a unit's statistics waits
-// for the unit's count and merges the partials itself, in double and in a
-// fixed order (no atomics on sums: the same bits from every run).  A wave is
-// small enough for its inputs to be in L2 still when the results read them
-// again, so HBM sees them once; where a unit alone is larger than that, the
-// results run backwards and find its second half there.
+// columns of an element (channels last).  Each set of CTAs takes units in
+// waves; its CTAs share a wave's items (equal parts of its units' voxels),
+// first for the sums, then for the results.  Every CTA leaves a partial for
+// each group of its item, and a CTA that needs a unit's statistics reads the
+// partials of all its items and merges them itself, in double and in a fixed
+// order (no atomics on sums: the same bits from every run).  A partial's words
+// are zero until they are written, so reading them is waiting for them: no
+// counter, no fence, no second hop.  The sets' waves together are small
+// enough for their inputs to be in L2 still when the results read them again,
+// so HBM sees them once; where a unit alone is larger than that, the results
+// run backwards and find the end of it there.
 //
-// A forward partial is (mean, M2), taken with the thread's own first value
-// subtracted: that shift is one of the summed values, so its distance from
+// A forward partial is the first and second moment about a value near the
+// mean, that value and the count; a thread sums about its own first value, and
+// that shift is one of the summed values, so its distance from
 // the mean is itself part of the variance, and M2's relative error stays
 // below the number of values a thread sums times 2^-24, whatever the data's
 // offset.
@@ -42,22 +45,23 @@ struct NormArgs {
   const void* bias;
   int32_t w_bf16;      // weight and bias are bf16 (else fp32)
   float* stats;        // (B, G, 2): mean, rstd
-  float4* part;        // a partial for each (unit, item, group of the unit):
-                       // mean, M2, count / sum w dz, sum w dz xh
+  float4* part;        // a partial for each (unit, group of the unit, item):
+                       // centre, second and first moment about it, count /
+                       // sum w dz, 0, sum w dz xh, 1.  Zeroed before the launch
   float2* chan;        // backward, where weight or bias want a gradient: sum dz,
                        // sum dz xh of each channel of each chunk
   void* dweight;       // (C,) or NULL, of the weight's type
   void* dbias;
-  uint32_t* sync;      // zeroed: items done, then those of each unit
+  uint32_t* done;      // backward, zeroed: items whose `chan` is written
   unsigned int* timeouts;  // where a wait that gave up is recorded, or NULL
   Feat f;
-  int64_t G, Cg;
+  uint32_t G, Cg;
   // the schedule (norm.cu)
-  int64_t units;
-  int64_t wave;    // units of a wave
-  int32_t items;   // work items of a unit
-  int32_t ugroups; // groups of a unit
-  int32_t ahead;   // sums of wave w + 1 before the results of wave w
+  uint32_t units;
+  uint32_t wave;   // units of a wave
+  uint32_t items;  // work items of a unit
+  uint32_t ugroups; // groups of a unit
+  uint32_t sets;    // the CTAs are so many sets, each taking every sets-th wave
   int32_t reverse; // results from the last voxel to the first
   double inv_n;    // 1 / values of a group
   float eps, slope;
@@ -69,8 +73,12 @@ __device__ __forceinline__ float norm_param(const void* p, int bf16, int64_t c, 
 }
 
 // ---------------------------------------------------------------------------
-// Activations, on pairs.  exp2 and the reciprocal are the hardware's (2 ulp),
-// well below the outputs' tolerance in either type.
+// Activations, on pairs.  exp2 and the reciprocal are the
+// hardware's (2 ulp), well below the outputs' tolerance in either type.  An SM
+// makes 16 of them a clock, so they are what an activation costs.  (Sharing
+// one reciprocal among four values, 1/a = b (1/(a b)), took 3 to 7 % off a
+// forward pass with silu, but a value's last bit then depends on its
+// neighbours', of other groups too; it was not kept.)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float exp2_hw(float x) {
   float r;
@@ -82,41 +90,67 @@ __device__ __forceinline__ float rcp_hw(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ F2 exp2_2(F2 t) { return f2(exp2_hw(t.x()), exp2_hw(t.y())); }
+
+__device__ __forceinline__ F2 rcp2(F2 t) { return f2(rcp_hw(t.x()), rcp_hw(t.y())); }
 
 __device__ __forceinline__ F2 sigmoid2(F2 z) {
-  const F2 t = mul2(z, f2(-1.44269504f));
-  const F2 d = add2(f2(exp2_hw(t.x), exp2_hw(t.y)), f2(1.0f));
-  return f2(rcp_hw(d.x), rcp_hw(d.y));
+  return rcp2(add2(exp2_2(mul2(z, f2(-1.44269504f))), f2(1.0f)));
 }
 
-__device__ __forceinline__ F2 normal_cdf2(F2 z) {
-  const F2 t = mul2(z, f2(0.70710678f));
-  return fma2(f2(erff(t.x), erff(t.y)), f2(0.5f), f2(0.5f));
+// The normal distribution function and exp(-z^2 / 2), by Hastings' formula
+// (Abramowitz and Stegun 7.1.26: erf(x) = 1 - (a1 t + .. + a5 t^5) exp(-x^2),
+// t = 1 / (1 + p x), |error| <= 1.5e-7) with x = |z| / sqrt(2); exp(-x^2) is the
+// density that the slope needs, so the slope costs no more exponentials.
+__device__ __forceinline__ F2 normal_tail2(F2 t, F2 e) {
+  // the coefficients are halved: 1 - cdf(|z|)
+  F2 q = fma2(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
+  q = fma2(q, t, f2(0.5f * 1.421413741f));
+  q = fma2(q, t, f2(0.5f * -0.284496736f));
+  q = fma2(q, t, f2(0.5f * 0.254829592f));
+  return mul2(mul2(q, t), e);
+}
+// 0.5 + sign(z) (0.5 - q)
+__device__ __forceinline__ F2 normal_side2(F2 z, F2 q) {
+  const F2 h = fma2(q, f2(-1.0f), f2(0.5f));
+  return add2(f2(copysignf(h.x(), z.x()), copysignf(h.y(), z.y())), f2(0.5f));
+}
+__device__ __forceinline__ F2 normal_cdf2(F2 z, F2& e) {
+  e = exp2_2(mul2(mul2(z, z), f2(-0.72134752f)));  // -log2(e) / 2
+  const F2 x = f2(fabsf(z.x()), fabsf(z.y()));
+  const F2 t = rcp2(fma2(x, f2(0.3275911f * 0.70710678f), f2(1.0f)));
+  return normal_side2(z, normal_tail2(t, e));
 }
 
+__device__ __forceinline__ F2 leaky2(F2 z, float slope) {
+  // slope 0: +0 for any negative z, infinite ones included
+  const F2 n = slope == 0.0f ? f2(0.0f) : mul2(z, f2(slope));
+  return f2(z.x() < 0.0f ? n.x() : z.x(), z.y() < 0.0f ? n.y() : z.y());
+}
+
+// act(z) and act'(z)
 template <int ACT>
 __device__ __forceinline__ F2 act_value2(F2 z, float slope) {
-  if constexpr (ACT == ACT_LEAKY) {
-    // slope 0: +0 for any negative z, infinite ones included
-    const F2 n = slope == 0.0f ? f2(0.0f) : mul2(z, f2(slope));
-    return f2(z.x < 0.0f ? n.x : z.x, z.y < 0.0f ? n.y : z.y);
-  }
+  if constexpr (ACT == ACT_LEAKY) return leaky2(z, slope);
   if constexpr (ACT == ACT_SILU) return mul2(z, sigmoid2(z));
-  if constexpr (ACT == ACT_GELU) return mul2(z, normal_cdf2(z));
+  if constexpr (ACT == ACT_GELU) {
+    F2 e;
+    return mul2(z, normal_cdf2(z, e));
+  }
   return z;
 }
-
 template <int ACT>
 __device__ __forceinline__ F2 act_slope2(F2 z, float slope) {
   if constexpr (ACT == ACT_LEAKY)
-    return f2(z.x > 0.0f ? 1.0f : slope, z.y > 0.0f ? 1.0f : slope);
+    return f2(z.x() > 0.0f ? 1.0f : slope, z.y() > 0.0f ? 1.0f : slope);
   if constexpr (ACT == ACT_SILU) {  // s + z s (1 - s)
     const F2 s = sigmoid2(z);
     return fma2(mul2(z, s), fma2(s, f2(-1.0f), f2(1.0f)), s);
   }
   if constexpr (ACT == ACT_GELU) {  // cdf + z pdf
-    const F2 t = mul2(mul2(z, z), f2(-0.72134752f));
-    return fma2(mul2(z, f2(0.39894228f)), f2(exp2_hw(t.x), exp2_hw(t.y)), normal_cdf2(z));
+    F2 e;
+    const F2 c = normal_cdf2(z, e);
+    return fma2(mul2(z, f2(0.39894228f)), e, c);
   }
   return f2(1.0f);
 }
@@ -136,47 +170,59 @@ struct PairConst {
 };
 
 // z = (x - mean) * a + bias with a = rstd * w; dx = a dz - c2 - (x - mean) c3.
-__device__ __forceinline__ PairConst pair_const(const NormArgs& a, const GroupStat& g,
-                                                int64_t c) {
-  const float w = norm_param(a.weight, a.w_bf16, c, 1.0f);
-  const float bias = norm_param(a.bias, a.w_bf16, c, 0.0f);
+__device__ __forceinline__ PairConst pair_const(const GroupStat& g, float w, float bias) {
   return {f2(-g.mean), f2(g.rstd * w), f2(bias), f2(-g.c2), f2(-g.c3)};
 }
 
-// The pair of results of x (and dy, its dropped elements zeroed); scale is
+// x -> the results of two pairs (dy: its dropped elements zeroed); scale is
 // dropout's, 1 without it.
 template <int DT, int ACT, bool DROP, bool BWD>
-__device__ __forceinline__ RawPair<DT> norm_pair(RawPair<DT> x, RawPair<DT> dy,
-                                                 const PairConst& k, float slope, float scale) {
-  const F2 xm = add2(pair_value<DT>(x), k.nmean);
-  const F2 z = fma2(xm, k.a, k.bias);
+__device__ __forceinline__ void norm_pairs(RawPair<DT>& x0, RawPair<DT>& x1, RawPair<DT> d0,
+                                           RawPair<DT> d1, const PairConst& k0,
+                                           const PairConst& k1, float slope, float scale) {
+  const F2 m0 = add2(pair_value<DT>(x0), k0.nmean), m1 = add2(pair_value<DT>(x1), k1.nmean);
+  F2 z0 = fma2(m0, k0.a, k0.bias), z1 = fma2(m1, k1.a, k1.bias);
   if constexpr (BWD) {
-    F2 dz = pair_value<DT>(dy);
-    if constexpr (ACT != ACT_NONE) dz = mul2(dz, act_slope2<ACT>(z, slope));
-    const F2 a = DROP ? mul2(k.a, f2(scale)) : k.a;
-    return pair_raw<DT>(fma2(a, dz, fma2(xm, k.nc3, k.nc2)));
+    F2 g0 = pair_value<DT>(d0), g1 = pair_value<DT>(d1);
+    if constexpr (ACT != ACT_NONE) {
+      g0 = mul2(g0, act_slope2<ACT>(z0, slope));
+      g1 = mul2(g1, act_slope2<ACT>(z1, slope));
+    }
+    const F2 a0 = DROP ? mul2(k0.a, f2(scale)) : k0.a, a1 = DROP ? mul2(k1.a, f2(scale)) : k1.a;
+    x0 = pair_raw<DT>(fma2(a0, g0, fma2(m0, k0.nc3, k0.nc2)));
+    x1 = pair_raw<DT>(fma2(a1, g1, fma2(m1, k1.nc3, k1.nc2)));
   } else {
-    F2 y = act_value2<ACT>(z, slope);
-    if constexpr (DROP) y = mul2(y, f2(scale));
-    return pair_raw<DT>(y);
+    z0 = act_value2<ACT>(z0, slope);
+    z1 = act_value2<ACT>(z1, slope);
+    if constexpr (DROP) {
+      z0 = mul2(z0, f2(scale));
+      z1 = mul2(z1, f2(scale));
+    }
+    x0 = pair_raw<DT>(z0);
+    x1 = pair_raw<DT>(z1);
   }
 }
 
-// Adds the pair to a forward (x about the shift) or backward (dz, dz (x -
-// mean), without dropout's scale) sum.
+// Adds two pairs to their forward (x about the shift) or backward (dz, dz (x -
+// mean), without dropout's scale) sums.
 template <int DT, int ACT, bool BWD>
-__device__ __forceinline__ void norm_add(RawPair<DT> x, RawPair<DT> dy, const PairConst& k,
-                                         float slope, F2& s0, F2& s1) {
-  const F2 xm = add2(pair_value<DT>(x), k.nmean);
+__device__ __forceinline__ void norm_add(RawPair<DT> x0, RawPair<DT> x1, RawPair<DT> d0,
+                                         RawPair<DT> d1, const PairConst& k0, const PairConst& k1,
+                                         float slope, F2& p0, F2& q0, F2& p1, F2& q1) {
+  const F2 m0 = add2(pair_value<DT>(x0), k0.nmean), m1 = add2(pair_value<DT>(x1), k1.nmean);
+  F2 g0 = m0, g1 = m1;
   if constexpr (BWD) {
-    F2 dz = pair_value<DT>(dy);
-    if constexpr (ACT != ACT_NONE) dz = mul2(dz, act_slope2<ACT>(fma2(xm, k.a, k.bias), slope));
-    s0 = add2(s0, dz);
-    s1 = fma2(dz, xm, s1);
-  } else {
-    s0 = add2(s0, xm);
-    s1 = fma2(xm, xm, s1);
+    g0 = pair_value<DT>(d0);
+    g1 = pair_value<DT>(d1);
+    if constexpr (ACT != ACT_NONE) {
+      g0 = mul2(g0, act_slope2<ACT>(fma2(m0, k0.a, k0.bias), slope));
+      g1 = mul2(g1, act_slope2<ACT>(fma2(m1, k1.a, k1.bias), slope));
+    }
   }
+  p0 = add2(p0, g0);
+  q0 = fma2(g0, m0, q0);
+  p1 = add2(p1, g1);
+  q1 = fma2(g1, m1, q1);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -191,136 +237,193 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // ===========================================================================
-// Counting and waiting.
+// Partials, from the CTA that has them to those that need them.
 // ===========================================================================
 constexpr unsigned long long NORM_WAIT_NS = 2000000000ull;
 
-__device__ __forceinline__ void count_release(uint32_t* p) {
-  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
-}
-__device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
-  uint32_t r;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(r) : "l"(p) : "memory");
-  return r;
-}
 __device__ __forceinline__ unsigned long long wall_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
+__device__ __forceinline__ void note_timeout(const NormArgs& a) {
+  if (a.timeouts != nullptr) atomicOr(a.timeouts, 1u);
+}
 
-// Waits, in every thread, until the counter reads n; false if it did not in
-// time.  Every CTA is resident and counts its items before it waits, so the
-// wait ends.
-static __device__ __noinline__ bool norm_wait(const NormArgs& a, const uint32_t* count,
-                                              uint32_t n) {
-  int ok = 1;
-  if (threadIdx.x == 0) {
-    unsigned long long t0 = 0;
-    while (load_acquire(count) != n) {
-      const unsigned long long t = wall_ns();
-      if (t0 == 0) t0 = t;
-      if (t - t0 > NORM_WAIT_NS) {
-        if (a.timeouts != nullptr) atomicOr(a.timeouts, 1u);
-        ok = 0;
-        break;
-      }
+// Two 8-byte words, each written and read whole, and each not zero: the low
+// halves are x and z, the high ones y with a set sign bit (a second moment, or
+// 0) and w (not 0).
+__device__ __forceinline__ void put_word(void* p, uint32_t lo, uint32_t hi) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"((uint64_t)hi << 32 | lo)
+               : "memory");
+}
+__device__ __forceinline__ uint2 look_word(const void* p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+}
+__device__ __forceinline__ void put_part(float4* p, float x, float y, float z, uint32_t w) {
+  put_word(p, __float_as_uint(x), __float_as_uint(y) | 0x80000000u);
+  put_word(reinterpret_cast<uint2*>(p) + 1, __float_as_uint(z), w);
+}
+__device__ __forceinline__ uint4 look_part(const float4* p) {
+  const uint2 a = look_word(p), b = look_word(reinterpret_cast<const uint2*>(p) + 1);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ bool is_part(const uint4& t) { return t.y != 0u && t.w != 0u; }
+
+// Looks until it is there; every CTA is resident and writes its partials
+// before it reads any, so it will be, or the wait ends without it (t0: the
+// wait's begin, 0 before).
+__device__ __forceinline__ void wait_part(const NormArgs& a, const float4* p, uint4& t,
+                                          unsigned long long& t0, bool& ok) {
+  while (!is_part(t) && ok) {
+    const unsigned long long now = wall_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > NORM_WAIT_NS) {
+      note_timeout(a);
+      ok = false;
     }
+    t = look_part(p);
+  }
+}
+
+// Sums over the partials k = first, first + step, ... of a group: forward,
+// the moments about the centre of the first one (k0); backward, the two sums.
+// False if one of them did not come.
+template <bool BWD>
+__device__ __forceinline__ bool sum_parts(const NormArgs& a, const float4* q, uint32_t first,
+                                          uint32_t step, double& s, double& m, double& k0) {
+  bool ok = true;
+  unsigned long long t0 = 0;
+  s = m = k0 = 0.0;
+  uint4 c = {};
+  if constexpr (!BWD) c = look_part(q);
+  for (uint32_t k = first; k < a.items; k += 4 * step) {
+    uint4 t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k + i * step < a.items) t[i] = look_part(q + k + i * step);
+    if constexpr (!BWD) {
+      wait_part(a, q, c, t0, ok);
+      k0 = (double)__uint_as_float(c.x);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k + i * step < a.items) {
+        wait_part(a, q + k + i * step, t[i], t0, ok);
+        const double x = (double)__uint_as_float(t[i].x), r = (double)__uint_as_float(t[i].z);
+        if constexpr (BWD) {
+          s += x;
+          m += r;
+        } else {
+          const double n = (double)t[i].w, d = x - k0;
+          s += n * d + r;
+          m += (double)__uint_as_float(t[i].y & 0x7FFFFFFFu) + d * (2.0 * r + n * d);
+        }
+      }
+  }
+  return ok;
+}
+
+// A group's partial from sums about k0 (forward), n values.
+__device__ __forceinline__ void put_moments(float4* p, double k0, double s, double m, double n) {
+  const float c = (float)k0 + (float)s * rcp_hw((float)n);
+  const double d = (double)c - k0;
+  put_part(p, c, (float)(m - d * (2.0 * s - n * d)), (float)(s - n * d), (uint32_t)n);
+}
+
+// A group's numbers from its merged partials.  `keep`: for the backward pass.
+template <bool BWD>
+__device__ __forceinline__ GroupStat group_stat(const NormArgs& a, int64_t at, double s, double m,
+                                                double k0, bool keep) {
+  float2* st = reinterpret_cast<float2*>(a.stats) + at;
+  const double d = s * a.inv_n;
+  if constexpr (BWD) {
+    const float2 t = *st;
+    return {t.x, t.y, t.y * (float)d, t.y * t.y * (float)(m * a.inv_n)};
+  } else {
+    const float var = (float)fmax(m * a.inv_n - d * d, 0.0) + a.eps;
+    const GroupStat r = {(float)(k0 + d), rsqrtf(isnan(m) ? __int_as_float(0x7FC00000) : var),
+                         0.0f, 0.0f};
+    if (keep) *st = make_float2(r.mean, r.rstd);
+    return r;
+  }
+}
+
+// The numbers of the unit's one group, in every thread; meet: 2 * FEAT_WARPS
+// entries that the CTA's previous call did not use.
+template <bool BWD>
+__device__ __forceinline__ bool norm_merge_one(const NormArgs& a, uint32_t u, bool keep,
+                                               double2* meet, GroupStat& r) {
+  double s, m, k0;
+  bool ok = sum_parts<BWD>(a, a.part + (int64_t)u * a.items, threadIdx.x, FEAT_THREADS, s, m, k0);
+  // a thread without a partial of its own has not seen the centre
+  s = warp_sum(s);
+  m = warp_sum(m);
+  if (threadIdx.x % 32 == 0) {
+    meet[threadIdx.x / 32] = make_double2(s, m);
+    if (threadIdx.x == 0) meet[FEAT_WARPS].x = k0;
+  }
+  ok = __syncthreads_and(ok);
+  s = m = 0.0;
+#pragma unroll
+  for (int i = 0; i < FEAT_WARPS; ++i) {
+    s += meet[i].x;
+    m += meet[i].y;
+  }
+  r = group_stat<BWD>(a, u, s, m, meet[FEAT_WARPS].x, keep && threadIdx.x == 0);
+  return ok;
+}
+
+// The numbers of the unit's groups in shared memory, a warp a group.
+template <bool BWD>
+__device__ __forceinline__ bool norm_merge(const NormArgs& a, uint32_t u, bool keep,
+                                           GroupStat* gs) {
+  bool ok = true;
+#pragma unroll 1
+  for (uint32_t g = threadIdx.x / 32; g < a.ugroups; g += FEAT_WARPS) {
+    const int64_t at = (int64_t)u * a.ugroups + g;
+    double s, m, k0;
+    ok = sum_parts<BWD>(a, a.part + at * a.items, threadIdx.x % 32, 32, s, m, k0) && ok;
+    s = warp_sum(s);
+    m = warp_sum(m);
+    if (threadIdx.x % 32 == 0) gs[g] = group_stat<BWD>(a, at, s, m, k0, keep);
   }
   return __syncthreads_and(ok) != 0;
 }
 
-// The item's partials are written.
-__device__ __forceinline__ void norm_arrive(const NormArgs& a, int64_t u) {
+// Backward: the item's `chan` is written, and all items' are.
+__device__ __forceinline__ void chan_done(const NormArgs& a) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    count_release(a.sync + 1 + u);
-    count_release(a.sync);
+    __threadfence();
+    asm volatile("red.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(a.done) : "memory");
   }
 }
-
-// A CTA's shared memory beside its rings.
-struct NormShared {
-  double2 meet[FEAT_THREADS];
-};
-
-// Partials of the unit's groups, merged: thread t < ugroups (looping) writes
-// group t's numbers to gs.  The threads split a group's partials and meet in
-// shared memory.  Partials are written by other CTAs of this launch, so they
-// are read through L2 (ld.global.cg).
-template <bool BWD>
-static __device__ __noinline__ void norm_merge(const NormArgs& a, int64_t u, int64_t stat0,
-                                               double2* meet, GroupStat* gs) {
-  const int ng = a.ugroups, gw = min(ng, FEAT_THREADS), parts = FEAT_THREADS / gw;
-  const int gi = threadIdx.x % gw, part = threadIdx.x / gw;
-  for (int g0 = 0; g0 < ng; g0 += gw) {
-    const int g = g0 + gi;
-    const float4* q = a.part + (u * a.items) * ng + g;
-    double s = 0.0, m2 = 0.0, k0 = 0.0;
-    const bool mine = part < parts && g < ng;
-    if (mine) {
-      if constexpr (!BWD) k0 = (double)__ldcg(q).x;
-#pragma unroll 4
-      for (int k = part; k < a.items; k += parts) {
-        const float4 t = __ldcg(q + (int64_t)k * ng);
-        if constexpr (BWD) {
-          s += (double)t.x;
-          m2 += (double)t.y;
-        } else {
-          const double n = (double)__float_as_uint(t.z), d = (double)t.x - k0;
-          s += n * d;
-          m2 += (double)t.y + n * d * d;
-        }
+__device__ __forceinline__ bool chan_wait(const NormArgs& a, uint32_t n) {
+  int ok = 1;
+  if (threadIdx.x == 0) {
+    const unsigned long long t0 = wall_ns();
+    uint32_t v;
+    do {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(a.done) : "memory");
+      if (v != n && wall_ns() - t0 > NORM_WAIT_NS) {
+        note_timeout(a);
+        ok = 0;
       }
-    }
-    __syncthreads();
-    meet[threadIdx.x] = make_double2(s, m2);
-    for (int m = parts; m > 1;) {
-      __syncthreads();
-      const int h = (m + 1) >> 1;
-      if (mine && part < m - h) {
-        double2 v = meet[threadIdx.x];
-        const double2 w = meet[threadIdx.x + h * gw];
-        v.x += w.x;
-        v.y += w.y;
-        meet[threadIdx.x] = v;
-      }
-      m = h;
-    }
-    if (mine && part == 0) {
-      const double2 v = meet[threadIdx.x];
-      GroupStat r;
-      float2* st = reinterpret_cast<float2*>(a.stats) + stat0 + g;
-      const double d = v.x * a.inv_n;
-      if constexpr (BWD) {
-        const float2 t = *st;
-        r.mean = t.x;
-        r.rstd = t.y;
-        r.c2 = t.y * (float)d;
-        r.c3 = t.y * t.y * (float)(v.y * a.inv_n);
-      } else {
-        const double var = v.y * a.inv_n - d * d;
-        r.mean = (float)(k0 + d);
-        r.rstd = __frcp_rn(__fsqrt_rn((float)(var < 0.0 ? 0.0 : var) + a.eps));
-        r.c2 = r.c3 = 0.0f;
-        // every CTA of the unit has the same; the backward pass wants it once
-        if (blockIdx.x == (unsigned)((u % a.wave) * a.items % gridDim.x))
-          *st = make_float2(r.mean, r.rstd);
-      }
-      gs[g] = r;
-    }
+    } while (v != n && ok);
   }
-  __syncthreads();
+  return __syncthreads_and(ok) != 0;
 }
 
-// cp.async of BYTES (4, 8, 16).
+// cp.async of BYTES (8, 16).
 template <int BYTES>
-__device__ __forceinline__ void cp_async(void* smem, const void* gmem) {
-  const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
+__device__ __forceinline__ void cp_async(uint32_t smem, const void* gmem) {
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s), "l"(gmem) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem), "l"(gmem) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(s), "l"(gmem), "n"(BYTES)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(smem), "l"(gmem), "n"(BYTES)
                  : "memory");
 }
 
@@ -328,60 +431,99 @@ __device__ __forceinline__ void cp_async(void* smem, const void* gmem) {
 // A thread's accesses, eight to a block, each thread's own ring of eight slots
 // in shared memory: while a block is worked on, the next one is on its way
 // (cp.async, no registers held).  Single elements are loaded into registers, a
-// block at a time, instead.
+// block at a time, instead.  What an access costs beside its arithmetic is
+// what bounds these kernels after HBM, so the addresses are a pointer to the
+// block plus j times a stride, and a block has one count of the accesses that
+// exist (negative or more than eight like none and eight).
 // ===========================================================================
 template <int DT, int VEC, bool BWD>
 struct Stream {
   static constexpr int BYTES = VEC * ESIZE<DT>;
-  const char *x, *dy;
-  char* slot;      // the thread's slot 0
-  uint32_t row;    // bytes between accesses of unit index distance
-  int n;           // indexes below n exist
-  int step;        // index distance inside a block
+  static constexpr int SLOT = FEAT_THREADS * BYTES;
+  const char *x, *dy;  // the block after the current one
+  char* slot;          // the thread's slot 0
+  uint32_t step;       // bytes between the accesses of a block
+  int64_t span;        // bytes between blocks, negative if backwards
+  int left, dec;       // the current block's count, what the next one has less
+  int blocks;          // of the thread
   Raw<DT, 1> rx[VEC == 1 ? 8 : 1], rd[VEC == 1 && BWD ? 8 : 1];
 
-  __device__ __forceinline__ int at(int r, int j) const { return r + j * step; }
-  __device__ __forceinline__ bool has(int r, int j) const { return at(r, j) < n && r >= 0; }
+  // To the last block, and from there backwards.
+  __device__ __forceinline__ void turn() {
+    const int n = blocks - 1;
+    if (n > 0) {
+      x += n * span;
+      dy += n * span;
+      left -= n * dec;
+    }
+    span = -span;
+    dec = -dec;
+  }
 
-  __device__ __forceinline__ void issue(int r, int j) {
+  // accesses j and j + 1 of the next block, `count` of which exist
+  __device__ __forceinline__ void issue2(int count, int j) {
     if constexpr (VEC > 1) {
-      if (has(r, j)) {
-        const uint64_t o = row_at(at(r, j), row);
-        cp_async<BYTES>(slot + j * FEAT_THREADS * BYTES, x + o);
-        if constexpr (BWD) cp_async<BYTES>(slot + (8 + j) * FEAT_THREADS * BYTES, dy + o);
-      }
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + j * SLOT;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (j + h < count) {
+          cp_async<BYTES>(to + h * SLOT, x + (uint64_t)(j + h) * step);
+          if constexpr (BWD) cp_async<BYTES>(to + (8 + h) * SLOT, dy + (uint64_t)(j + h) * step);
+        }
       cp_async_commit();
     }
   }
   // the first block
-  __device__ __forceinline__ void start(int r) {
+  __device__ __forceinline__ void start() {
+    if constexpr (VEC > 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) issue(r, j);
+      for (int j = 0; j < 8; j += 2) issue2(left, j);
+      x += span;
+      dy += span;
+    }
   }
-  // single elements: the whole block
-  __device__ __forceinline__ void fill(int r) {
+  // what the accesses lack that do not exist: zeros (a block ahead, like them)
+  __device__ __forceinline__ void zero(int count) {
+    if constexpr (VEC > 1) {
+      if (count < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j >= count) {
+            *reinterpret_cast<Raw<DT, VEC>*>(slot + j * SLOT) = {};
+            if constexpr (BWD) *reinterpret_cast<Raw<DT, VEC>*>(slot + (8 + j) * SLOT) = {};
+          }
+      }
+    }
+  }
+  // single elements: the whole current block
+  __device__ __forceinline__ void fill() {
     if constexpr (VEC == 1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         rx[j] = 0;
         if constexpr (BWD) rd[j] = 0;
-        if (has(r, j)) {
-          const uint64_t o = row_at(at(r, j), row);
-          rx[j] = raw_load<DT, 1>(x + o);
-          if constexpr (BWD) rd[j] = raw_load<DT, 1>(dy + o);
+        if (j < left) {
+          rx[j] = raw_load<DT, 1>(x + (uint64_t)j * step);
+          if constexpr (BWD) rd[j] = raw_load<DT, 1>(dy + (uint64_t)j * step);
         }
       }
     }
   }
+  // the current block is done with
+  __device__ __forceinline__ void next() {
+    x += span;
+    dy += span;
+    left -= dec;
+  }
   // accesses j and j + 1 of the block have arrived (those after them not)
   __device__ __forceinline__ void wait2() {
-    if constexpr (VEC > 1) cp_async_wait<6>();
+    if constexpr (VEC > 1) cp_async_wait<3>();
   }
   __device__ __forceinline__ Raw<DT, VEC> get_x(int j) const {
-    return *reinterpret_cast<const Raw<DT, VEC>*>(slot + j * FEAT_THREADS * BYTES);
+    return *reinterpret_cast<const Raw<DT, VEC>*>(slot + j * SLOT);
   }
   __device__ __forceinline__ Raw<DT, VEC> get_dy(int j) const {
-    return *reinterpret_cast<const Raw<DT, VEC>*>(slot + (8 + j) * FEAT_THREADS * BYTES);
+    return *reinterpret_cast<const Raw<DT, VEC>*>(slot + (8 + j) * SLOT);
   }
 };
 
@@ -389,31 +531,68 @@ struct Stream {
 template <int DT, int VEC, bool BWD>
 constexpr int RING_BYTES = VEC == 1 ? 0 : FEAT_THREADS * VEC * ESIZE<DT> * 8 * (BWD ? 2 : 1);
 
+// Single elements: accesses j .. j + 3 of the block, as two pairs.
+template <int DT, int ACT, bool BWD>
+__device__ __forceinline__ void single_add(const Stream<DT, 1, BWD>& st, int j,
+                                           const RawPair<DT>* d, const PairConst& k, float slope,
+                                           F2& s0, F2& s1) {
+  F2 p0 = f2(0.0f), q0 = p0, p1 = p0, q1 = p0;
+  norm_add<DT, ACT, BWD>(raw_join<DT>(st.rx[j], st.rx[j + 1]),
+                         raw_join<DT>(st.rx[j + 2], st.rx[j + 3]), d[0], d[1], k, k, slope, p0, q0,
+                         p1, q1);
+  // what does not exist adds nothing
+  const bool h0 = j < st.left, h1 = j + 1 < st.left, h2 = j + 2 < st.left, h3 = j + 3 < st.left;
+  s0 = add2(s0, f2(h0 ? p0.x() : 0.0f, h1 ? p0.y() : 0.0f));
+  s1 = add2(s1, f2(h0 ? q0.x() : 0.0f, h1 ? q0.y() : 0.0f));
+  s0 = add2(s0, f2(h2 ? p1.x() : 0.0f, h3 ? p1.y() : 0.0f));
+  s1 = add2(s1, f2(h2 ? q1.x() : 0.0f, h3 ? q1.y() : 0.0f));
+}
+template <int DT>
+__device__ __forceinline__ void single_store(char* out, uint32_t step, int j, int left,
+                                             RawPair<DT> y0, RawPair<DT> y1) {
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+    if (j + h < left)
+      raw_store<DT, 1>(out + (uint64_t)(j + h) * step, raw_half<DT>(h < 2 ? y0 : y1, h & 1));
+}
+
 // ===========================================================================
 // Channels last
 // ===========================================================================
+// Weight and bias of a pass's channel threadIdx.x, ahead of their use.
+struct ChanParam {
+  float w, bias;
+};
+__device__ __forceinline__ ChanParam chan_param(const NormArgs& a, int64_t c, int64_t end) {
+  if (c >= end) return {0.0f, 0.0f};
+  return {norm_param(a.weight, a.w_bf16, c, 1.0f), norm_param(a.bias, a.w_bf16, c, 0.0f)};
+}
+
 // The constants of a pass's channels in shared memory: plane by plane
 // (mean, a, bias, c2, c3, as PairConst has them), a thread's pair i at
 // (i * ncw + tx), so that neighbouring threads read neighbouring words.
-// sm: 5 * ncw * VEC floats.
+// sm: 5 * ncw * VEC floats; wt (backward sums): the weights, ncw * VEC.
 template <int VEC, bool COEF>
-__device__ __forceinline__ void last_consts(const NormArgs& a, const LastPlace& p, int64_t g0,
-                                            const GroupStat* gs, float* sm) {
+__device__ __forceinline__ void last_consts(const NormArgs& a, const LastPlace& p, uint32_t g0,
+                                            const GroupStat* gs, ChanParam own, float* sm,
+                                            float* wt) {
   constexpr int P = VEC > 1 ? 2 : 1;
   const int cw = a.f.ncw * VEC;
   const int64_t c0 = p.c - p.tx * VEC;
-  __syncthreads();
   for (int i = threadIdx.x; i < cw; i += FEAT_THREADS) {
     if (c0 + i < p.c_end) {
-      const int g = (int)((uint32_t)(c0 + i) / (uint32_t)a.Cg - (uint32_t)g0);
-      const PairConst q = pair_const(a, gs[g], c0 + i);
+      const uint32_t g = (uint32_t)(c0 + i) / a.Cg - g0;
+      const ChanParam cp = i < FEAT_THREADS ? own : chan_param(a, c0 + i, p.c_end);
+      const PairConst q = pair_const(gs[g], cp.w, cp.bias);
       float* to = sm + ((i % VEC / P) * a.f.ncw + i / VEC) * P + i % P;
-      to[0] = q.nmean.x;
-      to[cw] = q.a.x;
-      to[2 * cw] = q.bias.x;
+      to[0] = q.nmean.x();
+      to[cw] = q.a.x();
+      to[2 * cw] = q.bias.x();
       if constexpr (COEF) {
-        to[3 * cw] = q.nc2.x;
-        to[4 * cw] = q.nc3.x;
+        to[3 * cw] = q.nc2.x();
+        to[4 * cw] = q.nc3.x();
+      } else {
+        wt[i] = cp.w;
       }
     }
   }
@@ -447,121 +626,125 @@ template <int DT, int VEC, bool BWD, bool BLOCK>
 __device__ __forceinline__ Stream<DT, VEC, BWD> last_stream(const NormArgs& a, const LastPlace& p,
                                                             char* ring) {
   Stream<DT, VEC, BWD> s;
-  const int64_t base = last_base<DT>(a.f, p);
+  const uint32_t row = (uint32_t)a.f.C * ESIZE<DT>;
+  const int first = BLOCK ? p.ty * 8 : p.ty, span = p.nty * 8;
+  const int64_t base = last_base<DT>(a.f, p) + (int64_t)row_at(first, row);
   s.x = (const char*)a.x + base;
   s.dy = (const char*)a.dy + base;
   s.slot = ring + threadIdx.x * VEC * ESIZE<DT>;
-  s.row = (uint32_t)a.f.C * ESIZE<DT>;
-  s.n = p.on ? p.rows : 0;
-  s.step = BLOCK ? 1 : p.nty;
+  s.step = (BLOCK ? 1 : p.nty) * row;
+  s.span = (int64_t)row_at(span, row);
+  // rows that are left, or every nty-th of them
+  s.dec = BLOCK ? span : 8;
+  s.left = BLOCK ? p.rows - first : (p.rows - first + p.nty - 1) / p.nty;
+  if (!p.on) s.left = 0;
+  s.blocks = s.left > 0 ? (s.left + s.dec - 1) / s.dec : 0;
   return s;
 }
 
-template <bool BLOCK>
-__device__ __forceinline__ int last_first(const LastPlace& p) {
-  return BLOCK ? p.ty * 8 : p.ty;
-}
-
 // The sums of a pass (256 columns at most) of one item, added to the item's
-// groups.  sm: two planes of nty rows by cw channels, floats (2 *
-// FEAT_THREADS * VEC in all); acc: the groups' sums so far.
+// groups; the pass's first block is on its way, `first` is its address.
+// sm: two planes of nty rows by cw channels, floats (2 * FEAT_THREADS * VEC in
+// all), or the constants; meet: max(FEAT_THREADS, cw) entries; acc: the
+// groups' sums so far and their centres.
 template <int DT, int VEC, int ACT, bool DROP, bool BWD>
-__device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p, int64_t g0,
-                                          const GroupStat* gs, char* ring, float* sm,
+__device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
+                                          Stream<DT, VEC, BWD>& st, const char* first, uint32_t g0,
+                                          const GroupStat* gs, ChanParam own, float* sm, float* wt,
                                           double2* meet, double2* acc, bool first_pass) {
   constexpr bool BLOCK = BWD && DROP;
   constexpr int NP = VEC > 1 ? VEC / 2 : 1;  // pairs of channels, or of rows
-  Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, BLOCK>(a, p, ring);
-  const int span = p.nty * 8;
-  int r = last_first<BLOCK>(p);
-  st.start(r);
+  if constexpr (BWD) st.zero(st.left);
   F2 s0[NP], s1[NP];
   PairConst k[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) s0[i] = s1[i] = f2(0.0f);
   DropRate dr = {};
   if constexpr (BWD) {
-    last_consts<VEC, false>(a, p, g0, gs, sm);
+    if constexpr (DROP) dr = drop_rate(a.drop, p.b);
+    last_consts<VEC, false>(a, p, g0, gs, own, sm, wt);
 #pragma unroll
     for (int i = 0; i < NP; ++i) k[i] = last_const<VEC, false>(a, p, i, sm);
-    if constexpr (DROP) dr = drop_rate(a.drop, p.b);
   } else {
     // the thread's first row is its shift
 #pragma unroll
     for (int i = 0; i < NP; ++i) k[i] = {};
-    if (st.has(r, 0)) {
-      const Raw<DT, VEC> v = raw_load<DT, VEC>(st.x + row_at(r, st.row));
+    if (st.left > 0) {
+      const Raw<DT, VEC> v = raw_load<DT, VEC>(first);
       if constexpr (VEC > 1) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const F2 t = pair_value<DT>(raw_pair<DT, VEC>(v, i));
-          k[i].nmean = f2(-t.x, -t.y);
+          k[i].nmean = f2(-t.x(), -t.y());
         }
       } else {
         const F2 t = pair_value<DT>(raw_join<DT>(v, v));
-        k[0].nmean = f2(-t.x, -t.y);
+        k[0].nmean = f2(-t.x(), -t.y());
       }
     }
   }
 #pragma unroll 1
-  for (; r < st.n; r += span) {
+  for (int q = 0; q < st.blocks; ++q, st.next()) {
+    const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
     uint32_t keep[VEC];
-    if constexpr (BLOCK) last_keep<VEC>(a.f, dr, p, r, keep);
-    st.fill(r);
+    if constexpr (BLOCK) last_keep<VEC>(a.f, dr, p, q * p.nty * 8 + p.ty * 8, keep);
+    st.fill();
     if constexpr (VEC > 1) {
-#pragma unroll 1
-      for (int j = 0; j < 8; j += 2) {
-        st.wait2();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (st.has(r, j + h)) {
-            const Raw<DT, VEC> vx = st.get_x(j + h);
-            Raw<DT, VEC> vd = {};
-            if constexpr (BWD) vd = st.get_dy(j + h);
+      for (int j = 0; j < 8; ++j) {
+        if (j % 2 == 0) st.wait2();
+        const Raw<DT, VEC> vx = st.get_x(j);
+        Raw<DT, VEC> vd = {};
+        if constexpr (BWD) vd = st.get_dy(j);
+        // missing rows: a zero dy adds nothing; a zero x would
+        if (BWD || j < st.left) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              RawPair<DT> d = raw_pair<DT, VEC>(vd, i);
-              if constexpr (BLOCK) d = last_pair_keep<DT>(d, keep, i, h);
-              norm_add<DT, ACT, BWD>(raw_pair<DT, VEC>(vx, i), d, k[i], a.slope, s0[i], s1[i]);
+          for (int i = 0; i < NP; i += 2) {
+            RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
+            if constexpr (BLOCK) {
+              d0 = last_pair_keep<DT>(d0, keep, i, j);
+              d1 = last_pair_keep<DT>(d1, keep, i + 1, j);
             }
+            norm_add<DT, ACT, BWD>(raw_pair<DT, VEC>(vx, i), raw_pair<DT, VEC>(vx, i + 1), d0, d1,
+                                   k[i], k[i + 1], a.slope, s0[i], s1[i], s0[i + 1], s1[i + 1]);
           }
-        st.issue(r + span, j);
-        st.issue(r + span, j + 1);
-        if constexpr (BLOCK) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) keep[i] <<= 1;
         }
+        if (j % 2 == 1) st.issue2(more, j - 1);
       }
+      if constexpr (BWD) st.zero(more);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const bool h0 = st.has(r, j), h1 = st.has(r, j + 1);
-        RawPair<DT> d = {};
-        if constexpr (BWD) d = raw_join<DT>(st.rd[j], st.rd[j + 1]);
-        if constexpr (BLOCK) d = pair_keep<DT, 1, 3>(d, keep[0] << (j >> 1), keep[0] << (j >> 1));
-        F2 t0 = s0[0], t1 = s1[0];
-        norm_add<DT, ACT, BWD>(raw_join<DT>(st.rx[j], st.rx[j + 1]), d, k[0], a.slope, t0, t1);
-        s0[0] = f2(h0 ? t0.x : s0[0].x, h1 ? t0.y : s0[0].y);
-        s1[0] = f2(h0 ? t1.x : s1[0].x, h1 ? t1.y : s1[0].y);
+      for (int j = 0; j < 8; j += 4) {
+        RawPair<DT> d[2] = {};
+        if constexpr (BWD) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
+            const uint32_t w = BLOCK ? keep[0] << ((j >> 1) + h) : 0u;
+            if constexpr (BLOCK) d[h] = pair_keep<DT, 1, 3>(d[h], w, w);
+          }
+        }
+        single_add<DT, ACT, BWD>(st, j, d, k[0], a.slope, s0[0], s1[0]);
       }
     }
   }
   // threads -> channels
   const int cw = a.f.ncw * VEC, rows = p.rows;
   float* plane = sm + p.nty * cw;
-  const float n_own = (float)((rows - p.ty + p.nty - 1) / p.nty);  // forward: rows of this thread
-  const float inv = 1.0f / n_own;
+  // forward: thread row y has n0 rows of the item, one more below y1
+  const int n0 = rows / p.nty, y1 = rows - n0 * p.nty;
+  const float inv = 1.0f / (float)(n0 + (p.ty < y1 ? 1 : 0));
   __syncthreads();
   if (p.ty < p.nty) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int h = VEC > 1 ? i / 2 : 0;
-      const float t = VEC == 1 ? s0[0].x + s0[0].y : i & 1 ? s0[h].y : s0[h].x;
-      float u = t, w = VEC == 1 ? s1[0].x + s1[0].y : i & 1 ? s1[h].y : s1[h].x;
+      const float t = VEC == 1 ? s0[0].x() + s0[0].y() : i & 1 ? s0[h].y() : s0[h].x();
+      float u = t, w = VEC == 1 ? s1[0].x() + s1[0].y() : i & 1 ? s1[h].y() : s1[h].x();
       if constexpr (!BWD) {
         // a thread's (mean, M2); nothing when it had no row
         const float m = t * inv;
-        u = m - (i & 1 ? k[h].nmean.y : k[h].nmean.x);
+        u = m - (i & 1 ? k[h].nmean.y() : k[h].nmean.x());
         w = __fmaf_rn(-t, m, w);
       }
       sm[p.ty * cw + p.tx * VEC + i] = u;
@@ -569,79 +752,56 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
     }
   }
   __syncthreads();
+  // rows -> channel parts, about the mean of the group's first channel's first
+  // row; then, a warp a group, -> groups
   const int parts = cw >= FEAT_THREADS ? 1 : FEAT_THREADS / cw;
   const int64_t c0 = p.c - p.tx * VEC;
+  const int nch = (int)min((int64_t)cw, p.c_end - c0);  // channels of the pass
 #pragma unroll 1
   for (int cb = 0; cb < cw; cb += FEAT_THREADS) {
     const int ci = cb + (parts == 1 ? (int)threadIdx.x : (int)threadIdx.x % cw);
     const int part = parts == 1 ? 0 : threadIdx.x / cw;
-    const bool mine = part < parts && ci < cw && c0 + ci < p.c_end;
-    double u = 0.0, w = 0.0;
-    const double k0 = mine ? (double)sm[ci] : 0.0;
-    if (mine)
+    if (part >= parts || ci >= nch) continue;
+    double u = 0.0, w = 0.0, k0 = 0.0;
+    const uint32_t g = (uint32_t)(c0 + ci) / a.Cg;
+    if constexpr (!BWD) {
+      const int i0 = (int)max((int64_t)0, (int64_t)g * a.Cg - c0);
+      k0 = first_pass ? (double)sm[i0] : acc[2 * (g - g0) + 1].x;
+    }
 #pragma unroll 2
-      for (int y = part; y < p.nty && (BWD || y < rows); y += parts) {
-        const float q = sm[y * cw + ci], m2 = plane[y * cw + ci];
-        if constexpr (BWD) {
-          u += (double)q;
-          w += (double)m2;
-        } else {
-          const double n = (double)((rows - y + p.nty - 1) / p.nty), d = (double)q - k0;
-          u += n * d;
-          w += (double)m2 + n * d * d;
-        }
-      }
-    for (int m = parts; m > 1;) {
-      meet[threadIdx.x] = make_double2(u, w);
-      __syncthreads();
-      const int h = (m + 1) >> 1;
-      if (mine && part < m - h) {
-        u += meet[threadIdx.x + h * cw].x;
-        w += meet[threadIdx.x + h * cw].y;
-      }
-      __syncthreads();
-      m = h;
-    }
-    // (mean, M2) about k0, or the sums, of the channel in place of its row 0
-    if (mine && part == 0) {
+    for (int y = part; y < p.nty && (BWD || y < rows); y += parts) {
+      const float q = sm[y * cw + ci], m2 = plane[y * cw + ci];
       if constexpr (BWD) {
-        const double sc = DROP ? (double)dr.scale : 1.0;
-        const int64_t c = c0 + ci;
-        const float rstd = gs[(uint32_t)c / (uint32_t)a.Cg - (uint32_t)g0].rstd;
-        u *= sc;
-        w *= sc * (double)rstd;
-        if (a.chan != nullptr)
-          __stcg(a.chan + (p.b * a.f.nchunk + p.k) * a.f.C + c, make_float2((float)u, (float)w));
+        u += (double)q;
+        w += (double)m2;
       } else {
-        const double n = (double)rows, d = u / n;
-        w -= u * d;
-        u = k0 + d;
+        const double n = (double)(n0 + (y < y1 ? 1 : 0)), d = (double)q - k0;
+        u += n * d;
+        w += (double)m2 + n * d * d;
       }
-      sm[ci] = (float)u;
-      plane[ci] = (float)w;
     }
+    if constexpr (BWD) {
+      const double sc = DROP ? (double)dr.scale : 1.0;
+      u *= sc;
+      w *= sc * (double)gs[g - g0].rstd;
+    }
+    meet[part * cw + ci] = make_double2(u, w);
   }
   __syncthreads();
-  // channels -> groups, a warp a group
-  const int cend = (int)min((int64_t)cw, p.c_end - c0);
-  const int ga = (int)((uint32_t)c0 / (uint32_t)a.Cg), gb = (int)((uint32_t)(c0 + cend - 1) / (uint32_t)a.Cg);
+  const uint32_t ga = (uint32_t)c0 / a.Cg, gb = (uint32_t)(c0 + nch - 1) / a.Cg;
+  // a group is always the same warp's, so its sums are too
 #pragma unroll 1
-  for (int g = ga + (int)threadIdx.x / 32; g <= gb; g += FEAT_WARPS) {
+  for (uint32_t g = threadIdx.x / 32 + g0; g <= gb; g += FEAT_WARPS) {
+    if (g < ga) continue;
     const int i0 = (int)max((int64_t)0, (int64_t)g * a.Cg - c0);
-    const int i1 = (int)min((int64_t)cend, (int64_t)(g + 1) * a.Cg - c0);
+    const int ng = (int)min((int64_t)nch, (int64_t)(g + 1) * a.Cg - c0) - i0;
     double u = 0.0, w = 0.0;
-    const double k0 = first_pass || BWD ? (BWD ? 0.0 : (double)sm[i0]) : acc[2 * (g - g0) + 1].x;
-    for (int i = i0 + (int)threadIdx.x % 32; i < i1; i += 32) {
-      const double q = (double)sm[i], m2 = (double)plane[i];
-      if constexpr (BWD) {
-        const double wt = (double)norm_param(a.weight, a.w_bf16, c0 + i, 1.0f);
-        u += wt * q;
-        w += wt * m2;
-      } else {
-        const double n = (double)rows, e = q - k0;
-        u += n * e;
-        w += m2 + n * e * e;
-      }
+    for (int e = threadIdx.x % 32; e < ng * parts; e += 32) {
+      const int part = e / ng, i = i0 + e - part * ng;
+      const double2 t = meet[part * cw + i];
+      const double f = BWD ? (double)wt[i] : 1.0;
+      u += f * t.x;
+      w += f * t.y;
     }
     u = warp_sum(u);
     w = warp_sum(w);
@@ -649,81 +809,109 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
       double2* t = acc + 2 * (g - g0);
       if (first_pass) {
         t[0] = make_double2(u, w);
-        t[1] = make_double2(k0, 0.0);
+        t[1] = make_double2(BWD ? 0.0 : (double)sm[i0], 0.0);
       } else {
         t[0].x += u;
         t[0].y += w;
       }
     }
   }
-  __syncthreads();
+  if constexpr (BWD) {
+    if (a.chan != nullptr)
+      for (int ci = threadIdx.x; ci < nch; ci += FEAT_THREADS) {
+        double2 t = meet[ci];
+        for (int j = 1; j < parts; ++j) {
+          t.x += meet[j * cw + ci].x;
+          t.y += meet[j * cw + ci].y;
+        }
+        __stcg(a.chan + (p.b * a.f.nchunk + p.k) * a.f.C + c0 + ci,
+               make_float2((float)t.x, (float)t.y));
+      }
+  }
 }
 
-// y or dx of a pass of one item; `started`: its first block is on its way.
+// The item's partials, from the lanes that summed its groups.
+template <bool BWD>
+__device__ __forceinline__ void last_put(const NormArgs& a, const LastPlace& p, float4* part,
+                                         const double2* acc) {
+  if (threadIdx.x % 32 != 0) return;
+  for (uint32_t g = threadIdx.x / 32; g < a.ugroups; g += FEAT_WARPS) {
+    const double2 t = acc[2 * g];
+    if constexpr (BWD)
+      put_part(part + (int64_t)g * a.items, (float)t.x, 0.0f, (float)t.y, 1u);
+    else
+      put_moments(part + (int64_t)g * a.items, acc[2 * g + 1].x, t.x, t.y,
+                  (double)p.rows * (double)a.Cg);
+  }
+}
+
+// y or dx of a pass of one item; the pass's first block is on its way.
 template <int DT, int VEC, int ACT, bool DROP, bool BWD>
 __device__ __forceinline__ void last_apply(const NormArgs& a, const LastPlace& p,
-                                           Stream<DT, VEC, BWD>& st, int64_t g0,
-                                           const GroupStat* gs, float* sm) {
+                                           Stream<DT, VEC, BWD>& st, uint32_t g0,
+                                           const GroupStat* gs, ChanParam own, const DropRate& dr,
+                                           float* sm, float* wt) {
   constexpr int NP = VEC > 1 ? VEC / 2 : 1;
-  const int span = p.nty * 8, end = (p.rows + span - 1) / span * span;
-  const int dir = a.reverse ? -span : span;
-  int r = last_first<DROP>(p) + (a.reverse ? end - span : 0);
-  char* out = (char*)a.out + last_base<DT>(a.f, p);
-  last_consts<VEC, BWD>(a, p, g0, gs, sm);
+  last_consts<VEC, BWD>(a, p, g0, gs, own, sm, wt);
   if (!p.on) return;
-  DropRate dr = {};
-  if constexpr (DROP) dr = drop_rate(a.drop, p.b);
   const float scale = DROP ? dr.scale : 1.0f;
   PairConst k[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) k[i] = last_const<VEC, BWD>(a, p, i, sm);
+  // the result lies as x does; single elements are not a block ahead
+  char* out = (char*)a.out + (st.x - (const char*)a.x) - (VEC > 1 ? st.span : 0);
 #pragma unroll 1
-  for (int q = 0; q < end; q += span, r += dir) {
+  for (int q = 0; q < st.blocks; ++q, st.next(), out += st.span) {
+    const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
     uint32_t keep[VEC];
-    if constexpr (DROP) last_keep<VEC>(a.f, dr, p, r, keep);
-    st.fill(r);
+    if constexpr (DROP)
+      last_keep<VEC>(a.f, dr, p, (a.reverse ? st.blocks - 1 - q : q) * p.nty * 8 + p.ty * 8, keep);
+    st.fill();
     if constexpr (VEC > 1) {
-#pragma unroll 1
-      for (int j = 0; j < 8; j += 2) {
-        st.wait2();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (st.has(r, j + h)) {
-            Raw<DT, VEC> vx = st.get_x(j + h), vd = {};
-            if constexpr (BWD) vd = st.get_dy(j + h);
+      for (int j = 0; j < 8; ++j) {
+        if (j % 2 == 0) st.wait2();
+        Raw<DT, VEC> vx = st.get_x(j), vd = {};
+        if constexpr (BWD) vd = st.get_dy(j);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              RawPair<DT> d = raw_pair<DT, VEC>(vd, i);
-              if constexpr (BWD && DROP) d = last_pair_keep<DT>(d, keep, i, h);
-              RawPair<DT> y = norm_pair<DT, ACT, DROP, BWD>(raw_pair<DT, VEC>(vx, i), d, k[i],
-                                                            a.slope, scale);
-              if constexpr (DROP && !BWD) y = last_pair_keep<DT>(y, keep, i, h);
-              raw_set_pair<DT, VEC>(vx, i, y);
-            }
-            raw_store<DT, VEC>(out + row_at(st.at(r, j + h), st.row), vx);
+        for (int i = 0; i < NP; i += 2) {
+          RawPair<DT> y0 = raw_pair<DT, VEC>(vx, i), y1 = raw_pair<DT, VEC>(vx, i + 1);
+          RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
+          if constexpr (BWD && DROP) {
+            d0 = last_pair_keep<DT>(d0, keep, i, j);
+            d1 = last_pair_keep<DT>(d1, keep, i + 1, j);
           }
-        st.issue(r + dir, j);
-        st.issue(r + dir, j + 1);
-        if constexpr (DROP) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) keep[i] <<= 1;
+          norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d0, d1, k[i], k[i + 1], a.slope, scale);
+          if constexpr (DROP && !BWD) {
+            y0 = last_pair_keep<DT>(y0, keep, i, j);
+            y1 = last_pair_keep<DT>(y1, keep, i + 1, j);
+          }
+          raw_set_pair<DT, VEC>(vx, i, y0);
+          raw_set_pair<DT, VEC>(vx, i + 1, y1);
         }
+        if (j < st.left) raw_store<DT, VEC>(out + (uint64_t)j * st.step, vx);
+        if (j % 2 == 1) st.issue2(more, j - 1);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const uint32_t w = DROP ? keep[0] << (j >> 1) : 0u;
-        RawPair<DT> d = {};
+      for (int j = 0; j < 8; j += 4) {
+        RawPair<DT> d[2] = {};
+        const uint32_t w[2] = {DROP ? keep[0] << (j >> 1) : 0u, DROP ? keep[0] << ((j >> 1) + 1) : 0u};
         if constexpr (BWD) {
-          d = raw_join<DT>(st.rd[j], st.rd[j + 1]);
-          if constexpr (DROP) d = pair_keep<DT, 1, 3>(d, w, w);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
+            if constexpr (DROP) d[h] = pair_keep<DT, 1, 3>(d[h], w[h], w[h]);
+          }
         }
-        RawPair<DT> y = norm_pair<DT, ACT, DROP, BWD>(raw_join<DT>(st.rx[j], st.rx[j + 1]), d,
-                                                      k[0], a.slope, scale);
-        if constexpr (DROP && !BWD) y = pair_keep<DT, 1, 3>(y, w, w);
-        if (st.has(r, j)) raw_store<DT, 1>(out + row_at(st.at(r, j), st.row), raw_half<DT>(y, 0));
-        if (st.has(r, j + 1))
-          raw_store<DT, 1>(out + row_at(st.at(r, j + 1), st.row), raw_half<DT>(y, 1));
+        RawPair<DT> y0 = raw_join<DT>(st.rx[j], st.rx[j + 1]);
+        RawPair<DT> y1 = raw_join<DT>(st.rx[j + 2], st.rx[j + 3]);
+        norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d[0], d[1], k[0], k[0], a.slope, scale);
+        if constexpr (DROP && !BWD) {
+          y0 = pair_keep<DT, 1, 3>(y0, w[0], w[0]);
+          y1 = pair_keep<DT, 1, 3>(y1, w[1], w[1]);
+        }
+        single_store<DT>(out, st.step, j, st.left, y0, y1);
       }
     }
   }
@@ -733,29 +921,34 @@ __device__ __forceinline__ void last_apply(const NormArgs& a, const LastPlace& p
 // Channels first.  Item i of a group: 8 of its runs (channel, f.rows voxels),
 // one for each warp.  An access is 32 * VEC voxels of a warp.
 // ===========================================================================
-__device__ __forceinline__ bool first_item(const NormArgs& a, int64_t u, int i, FirstPlace& p) {
-  const int64_t run = (int64_t)i * FEAT_WARPS + threadIdx.x / 32;
+__device__ __forceinline__ void first_item(const NormArgs& a, uint32_t u, uint32_t i,
+                                           FirstPlace& p) {
+  const uint32_t run = i * FEAT_WARPS + threadIdx.x / 32;
+  const uint32_t cl = run / a.f.nchunk, k = run - cl * a.f.nchunk, b = u / a.G;
   p.lane = threadIdx.x % 32;
-  p.b = u / a.G;
-  const int64_t cl = run / a.f.nchunk;
-  p.k = run - cl * a.f.nchunk;
-  p.c = (u - p.b * a.G) * a.Cg + cl;
-  p.s0 = p.k * a.f.rows;
+  p.b = b;
+  p.k = k;
+  p.c = (u - b * a.G) * a.Cg + cl;
+  p.s0 = k * a.f.rows;
   p.n = cl < a.Cg ? (int)min(a.f.rows, a.f.S - p.s0) : 0;
   p.base = (p.b * a.f.C + p.c) * a.f.S + p.s0;
-  return cl < a.Cg;
 }
 
 template <int DT, int VEC, bool BWD>
 __device__ __forceinline__ Stream<DT, VEC, BWD> first_stream(const NormArgs& a,
                                                              const FirstPlace& p, char* ring) {
   Stream<DT, VEC, BWD> s;
-  s.x = (const char*)a.x + p.base * ESIZE<DT>;
-  s.dy = (const char*)a.dy + p.base * ESIZE<DT>;
+  constexpr int every = 32 * VEC;  // voxels of a warp's access
+  const int own = first_at<VEC>(p.lane, 0);
+  const int64_t base = (p.base + own) * ESIZE<DT>;
+  s.x = (const char*)a.x + base;
+  s.dy = (const char*)a.dy + base;
   s.slot = ring + threadIdx.x * VEC * ESIZE<DT>;
-  s.row = ESIZE<DT>;  // indexes are voxels
-  s.n = p.n;
-  s.step = 32 * VEC;
+  s.step = every * ESIZE<DT>;
+  s.span = 8 * every * ESIZE<DT>;
+  s.left = (p.n - own + every - 1) / every;  // rounds towards zero: none below it
+  s.dec = 8;
+  s.blocks = (p.n + 8 * every - 1) / (8 * every);  // of the warp
   return s;
 }
 
@@ -768,178 +961,200 @@ __device__ __forceinline__ void first_block_keep(const NormArgs& a, const DropRa
   if constexpr (VEC == 8) first_keep<VEC>(a.f, dr, p, s + FEAT_TILE, k + 1);
 }
 
+// The partial of one item.  meet: 2 * FEAT_WARPS entries that the CTA's
+// previous call did not use.
 template <int DT, int VEC, int ACT, bool DROP, bool BWD>
-__device__ __forceinline__ void first_sums(const NormArgs& a, const FirstPlace& p,
-                                           const GroupStat* gs, char* ring, double2* meet,
-                                           float4* part) {
+__device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const FirstPlace& p,
+                                           char* ring, double2* meet, float4* part) {
   Stream<DT, VEC, BWD> st = first_stream<DT, VEC, BWD>(a, p, ring);
-  const int own = first_at<VEC>(p.lane, 0);
-  constexpr int span = 256 * VEC;
-  st.start(own);
-  F2 s0 = f2(0.0f), s1 = f2(0.0f);
-  float shift = 0.0f;
+  const char* first = st.x;
+  const int cnt = max(st.left, 0) * VEC;  // the lane's voxels
+  st.start();
+  if constexpr (BWD) st.zero(st.left);
+  F2 s0 = f2(0.0f), s1 = f2(0.0f), u0 = f2(0.0f), u1 = f2(0.0f);
+  float shift = 0.0f, weight = 0.0f, rstd = 0.0f;
   PairConst k = {};
   DropRate dr = {};
   if constexpr (BWD) {
-    if (p.n > 0) {
-      k = pair_const(a, gs[0], p.c);
-      if constexpr (DROP) dr = drop_rate(a.drop, p.b);
-    }
+    const float2 t = reinterpret_cast<const float2*>(a.stats)[u_];
+    const ChanParam cp = chan_param(a, p.c, p.n > 0 ? a.f.C : 0);
+    k = pair_const({t.x, t.y, 0.0f, 0.0f}, cp.w, cp.bias);
+    weight = cp.w;
+    rstd = t.y;
+    if constexpr (DROP) dr = drop_rate(a.drop, p.b);
   } else {
-    if (own < p.n) shift = load_f(st.x, DT, own);
+    if (cnt > 0) shift = load_f(first, DT, 0);
     k.nmean = f2(-shift);
   }
 #pragma unroll 1
-  for (int s = 0; s < p.n; s += span) {
-    st.fill(s + own);
+  for (int q = 0; q < st.blocks; ++q, st.next()) {
+    const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
+    st.fill();
     if constexpr (VEC > 1) {
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < 8; j += 2) {
         uint32_t keep[2];
-        if constexpr (BWD && DROP) first_block_keep<VEC>(a, dr, p, s + j * 32 * VEC, keep);
+        if constexpr (BWD && DROP)
+          first_block_keep<VEC>(a, dr, p, (q * 8 + j) * 32 * VEC, keep);
         st.wait2();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (st.has(s + own, j + h)) {
-            const Raw<DT, VEC> vx = st.get_x(j + h);
-            Raw<DT, VEC> vd = {};
-            if constexpr (BWD) vd = st.get_dy(j + h);
+        for (int h = 0; h < 2; ++h) {
+          const Raw<DT, VEC> vx = st.get_x(j + h);
+          Raw<DT, VEC> vd = {};
+          if constexpr (BWD) vd = st.get_dy(j + h);
+          if (BWD || j + h < st.left) {
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-              RawPair<DT> d = raw_pair<DT, VEC>(vd, i);
-              if constexpr (BWD && DROP) d = pair_keep<DT, 1, 3>(d, keep[h] << i, keep[h] << i);
-              norm_add<DT, ACT, BWD>(raw_pair<DT, VEC>(vx, i), d, k, a.slope, s0, s1);
+            for (int i = 0; i < VEC / 2; i += 2) {
+              RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
+              if constexpr (BWD && DROP) {
+                d0 = pair_keep<DT, 1, 3>(d0, keep[h] << i, keep[h] << i);
+                d1 = pair_keep<DT, 1, 3>(d1, keep[h] << (i + 1), keep[h] << (i + 1));
+              }
+              norm_add<DT, ACT, BWD>(raw_pair<DT, VEC>(vx, i), raw_pair<DT, VEC>(vx, i + 1), d0,
+                                     d1, k, k, a.slope, s0, s1, u0, u1);
             }
           }
-        st.issue(s + own + span, j);
-        st.issue(s + own + span, j + 1);
+        }
+        st.issue2(more, j);
       }
+      if constexpr (BWD) st.zero(more);
     } else {
       uint32_t keep[8];
-      if constexpr (BWD && DROP) first_keep<VEC>(a.f, dr, p, s, keep);
+      if constexpr (BWD && DROP) first_keep<VEC>(a.f, dr, p, q * 8 * 32 * VEC, keep);
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const bool h0 = st.has(s + own, j), h1 = st.has(s + own, j + 1);
-        RawPair<DT> d = {};
-        if constexpr (BWD) d = raw_join<DT>(st.rd[j], st.rd[j + 1]);
-        if constexpr (BWD && DROP) d = pair_keep<DT, 3, 3>(d, keep[j], keep[j + 1]);
-        F2 t0 = s0, t1 = s1;
-        norm_add<DT, ACT, BWD>(raw_join<DT>(st.rx[j], st.rx[j + 1]), d, k, a.slope, t0, t1);
-        s0 = f2(h0 ? t0.x : s0.x, h1 ? t0.y : s0.y);
-        s1 = f2(h0 ? t1.x : s1.x, h1 ? t1.y : s1.y);
+      for (int j = 0; j < 8; j += 4) {
+        RawPair<DT> d[2] = {};
+        if constexpr (BWD) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
+            if constexpr (DROP)
+              d[h] = pair_keep<DT, 3, 3>(d[h], keep[j + 2 * h], keep[j + 2 * h + 1]);
+          }
+        }
+        single_add<DT, ACT, BWD>(st, j, d, k, a.slope, s0, s1);
       }
     }
   }
-  // lanes -> run -> item, in double
-  const int warp = threadIdx.x / 32;
-  double u, w;
-  double* shifts = reinterpret_cast<double*>(meet + 2 * FEAT_WARPS);
+  s0 = add2(s0, u0);
+  s1 = add2(s1, u1);
+  // lanes -> run -> item, in double; forward, a lane's (mean, M2) about the
+  // first lane's shift, a run's about the first run's
+  double u, w, k0 = 0.0;
   if constexpr (BWD) {
     const double sc = DROP ? (double)dr.scale : 1.0;
-    u = warp_sum((double)s0.x + (double)s0.y) * sc;
-    w = warp_sum((double)s1.x + (double)s1.y) * sc * (double)gs[0].rstd;
+    u = warp_sum((double)s0.x() + (double)s0.y()) * sc;
+    w = warp_sum((double)s1.x() + (double)s1.y()) * sc * (double)rstd;
     if (p.lane == 0 && p.n > 0 && a.chan != nullptr)
       __stcg(a.chan + (p.b * a.f.C + p.c) * a.f.nchunk + p.k, make_float2((float)u, (float)w));
-    const double wt = p.n > 0 ? (double)norm_param(a.weight, a.w_bf16, p.c, 1.0f) : 0.0;
-    u *= wt;
-    w *= wt;
+    u *= (double)weight;
+    w *= (double)weight;
   } else {
-    // a lane's (mean, M2), about the shift of the CTA's first lane
-    if (threadIdx.x == 0) shifts[0] = (double)shift;
-    __syncthreads();
-    int cnt = 0;
-#pragma unroll
-    for (int j = 0; j < (VEC == 1 ? 8 : 1); ++j) {
-      const int at = own + 32 * j;  // each access of VEC > 1 is whole
-      const int every = VEC == 1 ? FEAT_TILE : 32 * VEC;
-      cnt += at < p.n ? (p.n - at + every - 1) / every * VEC : 0;
-    }
+    k0 = (double)__shfl_sync(0xFFFFFFFFu, shift, 0);
     const double n = (double)cnt;
-    const float t0 = s0.x + s0.y, t1 = s1.x + s1.y;
+    const float t0 = s0.x() + s0.y(), t1 = s1.x() + s1.y();
     const float mt = cnt > 0 ? t0 / (float)cnt : 0.0f;
-    const double off = (double)shift - shifts[0] + (double)mt;
+    const double off = (double)shift - k0 + (double)mt;
     u = warp_sum(cnt > 0 ? n * off : 0.0);
     w = warp_sum(cnt > 0 ? (double)__fmaf_rn(-t0, mt, t1) + n * off * off : 0.0);
   }
+  const int warp = threadIdx.x / 32;
   if (p.lane == 0) {
     meet[warp] = make_double2(u, w);
-    meet[FEAT_WARPS + warp].x = (double)p.n;
+    meet[FEAT_WARPS + warp] = make_double2(k0, (double)p.n);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
     double n = 0.0;
     u = w = 0.0;
-    for (int i = 0; i < FEAT_WARPS; ++i) {
-      u += meet[i].x;
-      w += meet[i].y;
-      n += meet[FEAT_WARPS + i].x;
+    if (p.lane < FEAT_WARPS) {
+      const double2 t = meet[p.lane], e = meet[FEAT_WARPS + p.lane];
+      const double d = e.x - k0;
+      n = e.y;
+      u = t.x + n * d;
+      w = t.y + d * (2.0 * t.x + n * d);
+      if (n == 0.0) u = w = 0.0;
     }
-    if constexpr (BWD) {
-      __stcg(part, make_float4((float)u, (float)w, 0.0f, 0.0f));
-    } else {
-      const double d = u / n;
-      __stcg(part, make_float4((float)(shifts[0] + d), (float)(w - u * d),
-                               __uint_as_float((uint32_t)n), 0.0f));
+#pragma unroll
+    for (int o = FEAT_WARPS / 2; o > 0; o >>= 1) {
+      u += __shfl_down_sync(0xFFFFFFFFu, u, o);
+      w += __shfl_down_sync(0xFFFFFFFFu, w, o);
+      n += __shfl_down_sync(0xFFFFFFFFu, n, o);
+    }
+    if (p.lane == 0) {
+      if constexpr (BWD)
+        put_part(part, (float)u, 0.0f, (float)w, 1u);
+      else
+        put_moments(part, k0, u, w, n);
     }
   }
 }
 
 template <int DT, int VEC, int ACT, bool DROP, bool BWD>
 __device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace& p,
-                                            Stream<DT, VEC, BWD>& st, const GroupStat* gs) {
+                                            Stream<DT, VEC, BWD>& st, const PairConst& k,
+                                            const DropRate& dr) {
   if (p.n == 0) return;
-  const int own = first_at<VEC>(p.lane, 0);
-  constexpr int span = 256 * VEC;
-  const int end = (p.n + span - 1) / span * span, dir = a.reverse ? -span : span;
-  char* out = (char*)a.out + p.base * ESIZE<DT>;
-  const PairConst k = pair_const(a, gs[0], p.c);
-  DropRate dr = {};
-  if constexpr (DROP) dr = drop_rate(a.drop, p.b);
   const float scale = DROP ? dr.scale : 1.0f;
-  int s = a.reverse ? end - span : 0;
+  char* out = (char*)a.out + (st.x - (const char*)a.x) - (VEC > 1 ? st.span : 0);
 #pragma unroll 1
-  for (int q = 0; q < end; q += span, s += dir) {
-    st.fill(s + own);
+  for (int q = 0; q < st.blocks; ++q, st.next(), out += st.span) {
+    const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
+    const int s = (a.reverse ? st.blocks - 1 - q : q) * 8 * 32 * VEC;
+    st.fill();
     if constexpr (VEC > 1) {
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < 8; j += 2) {
         uint32_t keep[2];
         if constexpr (DROP) first_block_keep<VEC>(a, dr, p, s + j * 32 * VEC, keep);
         st.wait2();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (st.has(s + own, j + h)) {
-            Raw<DT, VEC> vx = st.get_x(j + h), vd = {};
-            if constexpr (BWD) vd = st.get_dy(j + h);
+        for (int h = 0; h < 2; ++h) {
+          Raw<DT, VEC> vx = st.get_x(j + h), vd = {};
+          if constexpr (BWD) vd = st.get_dy(j + h);
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-              RawPair<DT> d = raw_pair<DT, VEC>(vd, i);
-              if constexpr (BWD && DROP) d = pair_keep<DT, 1, 3>(d, keep[h] << i, keep[h] << i);
-              RawPair<DT> y =
-                  norm_pair<DT, ACT, DROP, BWD>(raw_pair<DT, VEC>(vx, i), d, k, a.slope, scale);
-              if constexpr (DROP && !BWD) y = pair_keep<DT, 1, 3>(y, keep[h] << i, keep[h] << i);
-              raw_set_pair<DT, VEC>(vx, i, y);
+          for (int i = 0; i < VEC / 2; i += 2) {
+            RawPair<DT> y0 = raw_pair<DT, VEC>(vx, i), y1 = raw_pair<DT, VEC>(vx, i + 1);
+            RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
+            const uint32_t w0 = DROP ? keep[h] << i : 0u, w1 = DROP ? keep[h] << (i + 1) : 0u;
+            if constexpr (BWD && DROP) {
+              d0 = pair_keep<DT, 1, 3>(d0, w0, w0);
+              d1 = pair_keep<DT, 1, 3>(d1, w1, w1);
             }
-            raw_store<DT, VEC>(out + (int64_t)st.at(s + own, j + h) * ESIZE<DT>, vx);
+            norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d0, d1, k, k, a.slope, scale);
+            if constexpr (DROP && !BWD) {
+              y0 = pair_keep<DT, 1, 3>(y0, w0, w0);
+              y1 = pair_keep<DT, 1, 3>(y1, w1, w1);
+            }
+            raw_set_pair<DT, VEC>(vx, i, y0);
+            raw_set_pair<DT, VEC>(vx, i + 1, y1);
           }
-        st.issue(s + own + dir, j);
-        st.issue(s + own + dir, j + 1);
+          if (j + h < st.left) raw_store<DT, VEC>(out + (j + h) * 32 * VEC * ESIZE<DT>, vx);
+        }
+        st.issue2(more, j);
       }
     } else {
       uint32_t keep[8];
       if constexpr (DROP) first_keep<VEC>(a.f, dr, p, s, keep);
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        RawPair<DT> d = {};
-        if constexpr (BWD) d = raw_join<DT>(st.rd[j], st.rd[j + 1]);
-        if constexpr (BWD && DROP) d = pair_keep<DT, 3, 3>(d, keep[j], keep[j + 1]);
-        RawPair<DT> y = norm_pair<DT, ACT, DROP, BWD>(raw_join<DT>(st.rx[j], st.rx[j + 1]), d, k,
-                                                      a.slope, scale);
-        if constexpr (DROP && !BWD) y = pair_keep<DT, 3, 3>(y, keep[j], keep[j + 1]);
-        if (st.has(s + own, j))
-          raw_store<DT, 1>(out + (int64_t)st.at(s + own, j) * ESIZE<DT>, raw_half<DT>(y, 0));
-        if (st.has(s + own, j + 1))
-          raw_store<DT, 1>(out + (int64_t)st.at(s + own, j + 1) * ESIZE<DT>, raw_half<DT>(y, 1));
+      for (int j = 0; j < 8; j += 4) {
+        RawPair<DT> d[2] = {};
+        if constexpr (BWD) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
+            if constexpr (DROP)
+              d[h] = pair_keep<DT, 3, 3>(d[h], keep[j + 2 * h], keep[j + 2 * h + 1]);
+          }
+        }
+        RawPair<DT> y0 = raw_join<DT>(st.rx[j], st.rx[j + 1]);
+        RawPair<DT> y1 = raw_join<DT>(st.rx[j + 2], st.rx[j + 3]);
+        norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d[0], d[1], k, k, a.slope, scale);
+        if constexpr (DROP && !BWD) {
+          y0 = pair_keep<DT, 3, 3>(y0, keep[j], keep[j + 1]);
+          y1 = pair_keep<DT, 3, 3>(y1, keep[j + 2], keep[j + 3]);
+        }
+        single_store<DT>(out, 32 * ESIZE<DT>, j, st.left, y0, y1);
       }
     }
   }
@@ -951,16 +1166,17 @@ template <bool LAST>
 static __device__ __noinline__ void norm_param_grads(const NormArgs& a, double2* meet) {
   const int ci = threadIdx.x % 8, part = threadIdx.x / 8;
   const int dt = a.w_bf16 ? BA_BF16 : BA_F32;
-  const int64_t n = a.f.B * a.f.nchunk;
+  const uint32_t n = (uint32_t)a.f.B * a.f.nchunk;
   for (int64_t c0 = (int64_t)blockIdx.x * 8; c0 < a.f.C; c0 += (int64_t)gridDim.x * 8) {
     const int64_t c = c0 + ci;
     double db = 0.0, dw = 0.0;
     if (c < a.f.C) {
 #pragma unroll 4
-      for (int64_t i = part; i < n; i += 32) {
+      for (uint32_t i = part; i < n; i += 32) {
         const float2 t = __ldcg(
-            a.chan + (LAST ? i * a.f.C + c
-                           : (i / a.f.nchunk * a.f.C + c) * a.f.nchunk + i % a.f.nchunk));
+            a.chan + (LAST ? (int64_t)i * a.f.C + c
+                           : ((int64_t)(i / a.f.nchunk) * a.f.C + c) * a.f.nchunk +
+                                 i % a.f.nchunk));
         db += (double)t.x;
         dw += (double)t.y;
       }
@@ -985,100 +1201,101 @@ static __device__ __noinline__ void norm_param_grads(const NormArgs& a, double2*
 template <int DT, bool LAST, int VEC, int ACT, bool DROP, bool BWD>
 __global__ void __launch_bounds__(FEAT_THREADS, 2)
     norm_kernel(const __grid_constant__ NormArgs a) {
-  // meet | group numbers | group sums | rings | planes or constants
+  // meet | group sums | group numbers | rings | weights | planes or constants
   extern __shared__ double2 norm_smem[];
   double2* meet = norm_smem;
-  double2* acc = meet + FEAT_THREADS;
+  double2* acc = meet + max(FEAT_THREADS, a.f.ncw * VEC);
   GroupStat* gs = reinterpret_cast<GroupStat*>(acc + 2 * a.ugroups);
   char* ring = reinterpret_cast<char*>(gs + a.ugroups);
-  float* sm = reinterpret_cast<float*>(ring + RING_BYTES<DT, VEC, BWD>);
-  const int64_t waves = (a.units + a.wave - 1) / a.wave;
-  for (int64_t w = 0; w < waves + a.ahead; ++w) {
-    if (w < waves) {
-      const int64_t u0 = w * a.wave, total = min(a.wave, a.units - u0) * a.items;
-      for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-        const int64_t u = u0 + t / a.items;
-        const int i = (int)(t % a.items);
-        float4* part = a.part + (u * a.items + i) * a.ugroups;
-        if constexpr (BWD) {
-          // mean and rstd of the unit's groups
-          __syncthreads();
-          const int64_t s0 = u * a.ugroups;
-          for (int g = threadIdx.x; g < a.ugroups; g += FEAT_THREADS) {
-            const float2 q = reinterpret_cast<const float2*>(a.stats)[s0 + g];
-            gs[g] = {q.x, q.y, 0.0f, 0.0f};
-          }
-          __syncthreads();
-        }
-        if constexpr (LAST) {
-          const int64_t g0 = (u % a.f.colblocks) * a.ugroups;
-          LastPlace p = last_place<VEC>(a.f, u / a.f.colblocks, i, u % a.f.colblocks);
-          bool first_pass = true;
-          while (true) {
-            last_sums<DT, VEC, ACT, DROP, BWD>(a, p, g0, gs, ring, sm, meet, acc, first_pass);
-            first_pass = false;
-            if (p.c - p.tx * VEC + a.f.ncw * VEC >= p.c_end) break;
-            p = last_next<VEC>(a.f, p);
-          }
-          for (int g = threadIdx.x; g < a.ugroups; g += FEAT_THREADS) {
-            const double2 q = acc[2 * g];
-            if constexpr (BWD) {
-              __stcg(part + g, make_float4((float)q.x, (float)q.y, 0.0f, 0.0f));
-            } else {
-              const double n = (double)p.rows * (double)a.Cg, d = q.x / n;
-              __stcg(part + g, make_float4((float)(acc[2 * g + 1].x + d), (float)(q.y - q.x * d),
-                                           __uint_as_float((uint32_t)n), 0.0f));
+  float* wt = reinterpret_cast<float*>(ring + RING_BYTES<DT, VEC, BWD>);
+  float* sm = wt + (a.f.ncw * VEC + 3) / 4 * 4;
+  const uint32_t waves = (a.units + a.wave - 1) / a.wave;
+  const unsigned ctas = gridDim.x / (unsigned)a.sets;
+  const unsigned set = blockIdx.x / ctas, own = blockIdx.x % ctas;
+  int turn = 0;  // channels first: the part of `meet` that is free
+  for (uint32_t w = set; w < waves; w += a.sets) {
+    const uint32_t u0 = w * a.wave, total = min(a.wave, a.units - u0) * a.items;
+    for (uint32_t t = own; t < total; t += ctas) {
+      const uint32_t u = u0 + t / a.items, i = t % a.items;
+      float4* part = a.part + (int64_t)u * a.ugroups * a.items + i;
+      if constexpr (LAST) {
+        const uint32_t b = u / a.f.colblocks, cb = u - b * a.f.colblocks, g0 = cb * a.ugroups;
+        LastPlace p = last_place<VEC>(a.f, b, i, cb);
+        bool first_pass = true;
+        while (true) {
+          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, BWD && DROP>(a, p, ring);
+          const char* first = st.x;
+          st.start();
+          ChanParam cp = {};
+          __syncthreads();  // the last use of the shared memory is over
+          if constexpr (BWD) {
+            cp = chan_param(a, p.c - p.tx * VEC + threadIdx.x, p.c_end);
+            if (first_pass) {
+              const float2* s = reinterpret_cast<const float2*>(a.stats) + (int64_t)u * a.ugroups;
+              for (uint32_t g = threadIdx.x; g < a.ugroups; g += FEAT_THREADS)
+                gs[g] = {s[g].x, s[g].y, 0.0f, 0.0f};
+              __syncthreads();
             }
           }
-        } else {
-          FirstPlace p;
-          first_item(a, u, i, p);
-          first_sums<DT, VEC, ACT, DROP, BWD>(a, p, gs, ring, meet, part);
+          last_sums<DT, VEC, ACT, DROP, BWD>(a, p, st, first, g0, gs, cp, sm, wt, meet, acc,
+                                             first_pass);
+          first_pass = false;
+          if (p.c - p.tx * VEC + a.f.ncw * VEC >= p.c_end) break;
+          p = last_next<VEC>(a.f, p);
         }
-        norm_arrive(a, u);
+        last_put<BWD>(a, p, part, acc);
+      } else {
+        FirstPlace p;
+        first_item(a, u, i, p);
+        first_sums<DT, VEC, ACT, DROP, BWD>(a, u, p, ring, meet + turn * 2 * FEAT_WARPS, part);
+        turn ^= 1;
+      }
+      if constexpr (BWD) {
+        if (a.chan != nullptr) chan_done(a);
       }
     }
-    const int64_t v = w - a.ahead;
-    if (v >= 0 && a.out != nullptr) {
-      const int64_t u0 = v * a.wave, total = min(a.wave, a.units - u0) * a.items;
-      for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-        const int64_t u = u0 + t / a.items;
-        const int i = (int)(t % a.items);
-        // the first block is on its way while the statistics are waited for
-        if constexpr (LAST) {
-          const int64_t g0 = (u % a.f.colblocks) * a.ugroups;
-          LastPlace p = last_place<VEC>(a.f, u / a.f.colblocks, i, u % a.f.colblocks);
-          bool first_pass = true;
-          while (true) {
-            Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, DROP>(a, p, ring);
-            const int span = p.nty * 8;
-            st.start(last_first<DROP>(p) + (a.reverse ? (p.rows - 1) / span * span : 0));
-            if (first_pass) {
-              if (!norm_wait(a, a.sync + 1 + u, (uint32_t)a.items)) return;
-              norm_merge<BWD>(a, u, u * a.ugroups, meet, gs);
-            }
-            first_pass = false;
-            last_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, g0, gs, sm);
-            if (p.c - p.tx * VEC + a.f.ncw * VEC >= p.c_end) break;
-            p = last_next<VEC>(a.f, p);
-          }
-        } else {
-          FirstPlace p;
-          first_item(a, u, i, p);
-          Stream<DT, VEC, BWD> st = first_stream<DT, VEC, BWD>(a, p, ring);
-          constexpr int span = 256 * VEC;
-          st.start(first_at<VEC>(p.lane, 0) +
-                   (a.reverse && p.n > 0 ? (p.n - 1) / span * span : 0));
-          if (!norm_wait(a, a.sync + 1 + u, (uint32_t)a.items)) return;
-          norm_merge<BWD>(a, u, u, meet, gs);
-          first_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, gs);
+    if (a.out == nullptr) continue;
+    for (uint32_t t = own; t < total; t += ctas) {
+      const uint32_t u = u0 + t / a.items, i = t % a.items;
+      // the first block and what else the results need are on their way while
+      // the statistics are waited for
+      if constexpr (LAST) {
+        const uint32_t b = u / a.f.colblocks, cb = u - b * a.f.colblocks, g0 = cb * a.ugroups;
+        LastPlace p = last_place<VEC>(a.f, b, i, cb);
+        DropRate dr = {};
+        if constexpr (DROP) dr = drop_rate(a.drop, p.b);
+        bool first_pass = true;
+        while (true) {
+          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, DROP>(a, p, ring);
+          if (a.reverse) st.turn();
+          st.start();
+          const ChanParam cp = chan_param(a, p.c - p.tx * VEC + threadIdx.x, p.c_end);
+          __syncthreads();  // the last use of the shared memory is over
+          if (first_pass && !norm_merge<BWD>(a, u, i == 0, gs)) return;
+          first_pass = false;
+          last_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, g0, gs, cp, dr, sm, wt);
+          if (p.c - p.tx * VEC + a.f.ncw * VEC >= p.c_end) break;
+          p = last_next<VEC>(a.f, p);
         }
+      } else {
+        FirstPlace p;
+        first_item(a, u, i, p);
+        Stream<DT, VEC, BWD> st = first_stream<DT, VEC, BWD>(a, p, ring);
+        if (a.reverse) st.turn();
+        st.start();
+        const ChanParam cp = chan_param(a, p.c, p.n > 0 ? a.f.C : 0);
+        DropRate dr = {};
+        if constexpr (DROP) dr = drop_rate(a.drop, p.b);
+        GroupStat g;
+        if (!norm_merge_one<BWD>(a, u, i == 0, meet + (4 + turn * 2) * FEAT_WARPS, g)) return;
+        turn ^= 1;
+        first_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, pair_const(g, cp.w, cp.bias), dr);
       }
     }
   }
   if constexpr (BWD) {
     if (a.chan != nullptr) {
-      if (!norm_wait(a, a.sync, (uint32_t)(a.units * a.items))) return;
+      if (!chan_wait(a, a.units * a.items)) return;
       norm_param_grads<LAST>(a, meet);
     }
   }

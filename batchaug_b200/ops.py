@@ -418,7 +418,9 @@ def _feature_map(x: torch.Tensor, name: str):
     if x.dim() != 5:
         raise ValueError(f"expected a (B,C,H,W,D) tensor, got shape {tuple(x.shape)}")
     if x.is_contiguous():
-        return x, L.BA_CHANNELS_FIRST
+        # one voxel: both layouts at once, and its channels are the long axis
+        one = x.shape[2] * x.shape[3] * x.shape[4] == 1
+        return x, L.BA_CHANNELS_LAST if one else L.BA_CHANNELS_FIRST
     if x.is_contiguous(memory_format=torch.channels_last_3d):
         return x, L.BA_CHANNELS_LAST
     return x.contiguous(), L.BA_CHANNELS_FIRST
@@ -456,39 +458,41 @@ def _drop_params(x: torch.Tensor, p, seed, name: str):
     return p, p_elem, int(seed) & 0xFFFFFFFFFFFFFFFF, seed_dev
 
 
-def _on(device: torch.device):
-    """The device made current, when it is another one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(fn, name: str, nbytes: int, device: torch.device, *args) -> None:
+    """One C entry on the device's current stream, with the device current."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch(fn, name, nbytes, device, *args)
+    tok = _timing.begin(name, nbytes, device)
+    st = fn(*args, L.stream_ptr(device))
+    if st:
+        L.check(st, name)
+    _timing.end(tok)
 
 
-def _dropout_call(x, layout, spec, p_elem, mask, seed_dev, out=None):
-    out = torch.empty_like(x) if out is None else out
-    p, seed, elem_offset, flags = spec
-    B, C, H, W, D = x.shape
-    d = L.DropoutDesc(x.data_ptr(), out.data_ptr(), B, C, H, W, D, L.dtype_code(x), layout, flags,
-                      p, L.ptr(p_elem), L.ptr(mask), seed, L.ptr(seed_dev), elem_offset)
-    with _on(x.device):
-        tok = _timing.begin("ba_dropout", 2 * x.numel() * x.element_size(), x.device)
-        L.check(L.lib.ba_dropout(ctypes.byref(d), L.stream_ptr(x.device)), "ba_dropout")
-        _timing.end(tok)
+def _dropout_call(x, desc):
+    out = torch.empty_like(x)
+    desc.src, desc.dst = x.data_ptr(), out.data_ptr()
+    _launch(L.lib.ba_dropout, "ba_dropout", 2 * x.numel() * x.element_size(), x.device,
+            ctypes.byref(desc))
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, layout, spec, p_elem, mask, seed_dev):
-        ctx.layout, ctx.spec = layout, spec
-        ctx.save_for_backward(p_elem, mask, seed_dev)
-        return _dropout_call(x, layout, spec, p_elem, mask, seed_dev)
+    def forward(ctx, x, desc, layout, tensors):
+        # the tensors behind the descriptor's addresses, if it has any
+        ctx.save_for_backward(*tensors)
+        ctx.desc, ctx.layout = desc, layout
+        return _dropout_call(x, desc)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        ctx.saved_tensors  # raises if one of them was written to since
         # the same draw on the gradient
-        dx = _dropout_call(_like(dy, dy, ctx.layout), ctx.layout, ctx.spec, *ctx.saved_tensors)
-        return dx, None, None, None, None, None
+        desc = L.DropoutDesc.from_buffer_copy(ctx.desc)
+        return _dropout_call(_like(dy, dy, ctx.layout), desc), None, None, None
 
 
 def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
@@ -506,65 +510,57 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     depend on (seed, elem_offset + element, channel, voxel) only, not on
     the memory layout, which the result shares with x."""
     x, layout = _feature_map(x, "x")
-    L.dtype_code(x)
+    dtype = L.dtype_code(x)
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "dropout")
     m = _dev_mask(mask, x.shape[0], x.device)
     flags = (L.BA_DROPOUT_CHANNEL if channelwise else 0) | (L.BA_DROPOUT_RESCALE if rescale else 0)
-    spec = (p, seed, int(elem_offset), flags)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, layout, spec, p_elem, m, seed_dev)
-    return _dropout_call(x, layout, spec, p_elem, m, seed_dev)
-
-
-def _norm_desc(x, layout, spec, weight, bias, p_elem, seed_dev, stats):
-    groups, act, eps, slope, p, seed, elem_offset = spec
     B, C, H, W, D = x.shape
-    param = weight if weight is not None else bias
-    return L.NormDesc(x.data_ptr(), None, None, L.ptr(weight), L.ptr(bias), None, None,
-                      stats.data_ptr(), B, C, H, W, D, groups, L.dtype_code(x), layout,
-                      L.BA_F32 if param is None else L.dtype_code(param), act, eps, slope, p, 0,
-                      L.ptr(p_elem), seed, L.ptr(seed_dev), elem_offset)
+    desc = L.DropoutDesc(None, None, B, C, H, W, D, dtype, layout, flags, p, L.ptr(p_elem),
+                         L.ptr(m), seed, L.ptr(seed_dev), int(elem_offset))
+    if torch.is_grad_enabled() and x.requires_grad:
+        tensors = [t for t in (p_elem, m, seed_dev) if t is not None]
+        return _Dropout.apply(x, desc, layout, tensors)
+    return _dropout_call(x, desc)
 
 
-def _norm_run(d, backward, name, nbytes, device):
-    with _on(device):
-        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(d), backward)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        tok = _timing.begin(name, nbytes, device)
-        fn = L.lib.ba_norm_backward if backward else L.lib.ba_norm_forward
-        L.check(fn(ctypes.byref(d), L.ptr(ws), size, L.stream_ptr(device)), name)
-        _timing.end(tok)
+def _norm_call(fn, name, desc, backward, nbytes, device):
+    size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), backward)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _launch(fn, name, nbytes, device, ctypes.byref(desc), L.ptr(ws), size)
 
 
-def _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev):
+def _norm_forward(x, desc, groups):
     y = torch.empty_like(x)
-    stats = torch.empty((x.shape[0], spec[0], 2), dtype=torch.float32, device=x.device)
-    d = _norm_desc(x, layout, spec, weight, bias, p_elem, seed_dev, stats)
-    d.out = y.data_ptr()
-    _norm_run(d, 0, "ba_norm_forward", 2 * x.numel() * x.element_size(), x.device)
+    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+    desc.out, desc.stats = y.data_ptr(), stats.data_ptr()
+    _norm_call(L.lib.ba_norm_forward, "ba_norm_forward", desc, 0,
+               2 * x.numel() * x.element_size(), x.device)
     return y, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, layout, spec, p_elem, seed_dev):
-        y, stats = _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev)
-        ctx.layout, ctx.spec = layout, spec
-        ctx.save_for_backward(x, weight, bias, p_elem, seed_dev, stats)
+    def forward(ctx, x, weight, bias, desc, groups, layout, tensors):
+        y, stats = _norm_forward(x, desc, groups)
+        ctx.desc, ctx.layout = desc, layout
+        # x, the parameters, and what else the descriptor points to
+        ctx.save_for_backward(x, weight, bias, stats, *tensors)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, p_elem, seed_dev, stats = ctx.saved_tensors
+        x, weight, bias = ctx.saved_tensors[:3]
         dy = _like(dy, x, ctx.layout)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        d = _norm_desc(x, ctx.layout, ctx.spec, weight, bias, p_elem, seed_dev, stats)
-        d.dy, d.out, d.dweight, d.dbias = dy.data_ptr(), L.ptr(dx), L.ptr(dw), L.ptr(db)
-        _norm_run(d, 1, "ba_norm_backward", 3 * x.numel() * x.element_size(), x.device)
+        desc = L.NormDesc.from_buffer_copy(ctx.desc)
+        desc.dy, desc.out = dy.data_ptr(), L.ptr(dx)
+        desc.dweight, desc.dbias = L.ptr(dw), L.ptr(db)
+        _norm_call(L.lib.ba_norm_backward, "ba_norm_backward", desc, 1,
+                   3 * x.numel() * x.element_size(), x.device)
         return dx, dw, db, None, None, None, None
 
 
@@ -594,7 +590,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     default.  x may be contiguous or in torch.channels_last_3d, and the
     result is laid out as it is."""
     x, layout = _feature_map(x, "x")
-    L.dtype_code(x)
+    dtype = L.dtype_code(x)
     num_groups = int(num_groups)
     if num_groups < 1 or x.shape[1] % num_groups:
         raise ValueError(f"group_norm: {num_groups} groups do not divide {x.shape[1]} channels")
@@ -605,13 +601,19 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "group_norm")
-    spec = (num_groups, L.ACTIVATIONS[activation], float(eps), float(negative_slope), p, seed,
-            int(elem_offset))
+    B, C, H, W, D = x.shape
+    param = weight if weight is not None else bias
+    desc = L.NormDesc(x.data_ptr(), None, None, L.ptr(weight), L.ptr(bias), None, None, None, B, C,
+                      H, W, D, num_groups, dtype, layout,
+                      L.BA_F32 if param is None else L.dtype_code(param),
+                      L.ACTIVATIONS[activation], eps, negative_slope, p, 0, L.ptr(p_elem), seed,
+                      L.ptr(seed_dev), int(elem_offset))
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _GroupNorm.apply(x, weight, bias, layout, spec, p_elem, seed_dev)
-    return _norm_forward(x, layout, spec, weight, bias, p_elem, seed_dev)[0]
+        tensors = [t for t in (p_elem, seed_dev) if t is not None]
+        return _GroupNorm.apply(x, weight, bias, desc, num_groups, layout, tensors)
+    return _norm_forward(x, desc, num_groups)[0]
 
 
 def host_rand_affine(u, prob, a, b, c, present, groups, spatial_shape, mask, affine, theta):

@@ -376,3 +376,26 @@ def test_refusals(ba):
     (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("shape, groups", [((1, 300, 1, 2, 5), 1), ((1, 8, 40, 40, 40), 1),
+                                           ((2, 64, 24, 24, 24), 8), ((1, 2, 96, 64, 64), 2)])
+def test_statistics_of_many_parts(ba, shape, groups, layout):
+    """Units whose partials come from many CTAs: the same bits from launches
+    that find the caches cold and from ones that do not, and the definition's
+    statistics each time."""
+    junk = torch.empty(48 << 20, device="cuda")
+    x = _x(shape, torch.float32, layout, offset=2.0)
+    r = x.double().reshape(shape[0], groups, -1)
+    ref = (r - r.mean(-1, keepdim=True)) / torch.sqrt(r.var(-1, correction=0, keepdim=True) + 1e-5)
+    ref = ref.reshape(shape)
+    first = ba.ops.group_norm(x, groups)
+    # as K above: 160 u R rstd, R rstd below 8 here, plus 4 u M rstd
+    assert float((first.double() - ref).abs().max()) <= 160 * U * 8 + 4 * U * 16 + 160 * U * 8
+    for i in range(40):
+        if i % 2:
+            junk.zero_()
+        assert torch.equal(ba.ops.group_norm(x, groups), first)
+    from batchaug_b200 import _lib as L
+    L.wait_status(x.device)
