@@ -18,7 +18,7 @@ from . import _lib  # noqa: F401  (loads libbatchaug_b200.so or raises ImportErr
 from ._rng import get_shard, set_shard, shard
 from .base import BatchDictTransform, BatchTransform
 from .compose import Compose
-from .ops import resample_exact, set_resample_exact
+from .ops import dropout, group_norm, resample_exact, set_resample_exact
 from .geometric import (
     Rand3DElastic,
     Rand3DElasticd,
@@ -36,6 +36,8 @@ from .geometric import (
     RandZoomd,
 )
 from .intensity import (
+    NormalizeIntensity,
+    NormalizeIntensityd,
     RandAdjustContrast,
     RandAdjustContrastd,
     RandBiasField,
@@ -58,6 +60,8 @@ from .intensity import (
     RandSimulateLowResolutiond,
     RandStdShiftIntensity,
     RandStdShiftIntensityd,
+    RandVoxelDropout,
+    RandVoxelDropoutd,
     ScaleIntensity,
     ScaleIntensityd,
 )
@@ -93,4 +97,7 @@ __all__ = [
     "RandShiftIntensityd", "RandSimulateLowResolution", "RandSimulateLowResolutiond",
     "RandStdShiftIntensity", "RandStdShiftIntensityd",
     "ScaleIntensity", "ScaleIntensityd",
+    # network side, without counterparts in the reference
+    "NormalizeIntensity", "NormalizeIntensityd", "RandVoxelDropout", "RandVoxelDropoutd",
+    "dropout", "group_norm",
 ]

@@ -26,7 +26,7 @@ BA_MAX_KEYS = 8
 BA_MAX_OPS = 8
 
 BA_OP_NOISE, BA_OP_CONTRAST, BA_OP_SCALE, BA_OP_SHIFT, BA_OP_BIAS_FIELD, BA_OP_RESCALE = 1, 2, 3, 4, 5, 6
-BA_OP_RICIAN, BA_OP_STD_SHIFT, BA_OP_FIXED_MEAN = 7, 8, 9
+BA_OP_RICIAN, BA_OP_STD_SHIFT, BA_OP_FIXED_MEAN, BA_OP_DROPOUT = 7, 8, 9, 10
 BA_NOISE_PHILOX = 0x1
 BA_RICIAN_PHILOX, BA_RICIAN_RELATIVE = 0x1, 0x2
 BA_STD_NONZERO, BA_STAT_CHANNEL = 0x2, 0x4

@@ -43,6 +43,7 @@ S_STD_SHIFT = 14
 S_FIXED_MEAN = 15
 S_SHARPEN = 16
 S_LOWRES = 17
+S_DROPOUT = 18
 
 
 def set_shard(element_offset: int = 0, global_batch: int | None = None) -> None:

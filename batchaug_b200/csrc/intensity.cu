@@ -27,6 +27,7 @@
 #include <vector>
 
 #include "ba_common.cuh"
+#include "dropout.cuh"
 #include "philox.cuh"
 
 namespace ba {
@@ -197,7 +198,21 @@ __device__ __forceinline__ float moment_std(const double* m, int64_t g, int64_t 
   return (float)sqrt(v);
 }
 
-template <int DT>
+// A dropout's constants: its rate and key in the bits of k0 .. h1.
+__device__ __forceinline__ DropRate drop_of(const OpConst& k) {
+  DropRate r;
+  r.scale = k.k0;
+  r.hi = __float_as_uint(k.k1);
+  r.lo = __float_as_uint(k.k2);
+  r.k0 = __float_as_uint(k.k3);
+  r.k1 = __float_as_uint(k.k4);
+  r.e_lo = k.h0;
+  r.e_hi = k.h1;
+  return r;
+}
+
+// ANY: the sequence may hold a dropout (kept out of the other kernels).
+template <int DT, bool ANY>
 __device__ __forceinline__ void resolve_op(const ChainArgs& a, int oi, int64_t b, int64_t c,
                                            OpConst& o) {
   const OpArgs& op = a.ops[oi];
@@ -271,6 +286,22 @@ __device__ __forceinline__ void resolve_op(const ChainArgs& a, int oi, int64_t b
       o.k1 = 1.0f + op.param[b];
       break;
     }
+    case BA_OP_DROPOUT:
+      if constexpr (ANY) {
+        const DropArgs da = {0.0f, op.param, op.mask, op.seed_lo, op.seed_hi, nullptr,
+                             op.elem_offset, (op.flags & BA_DROPOUT_RESCALE) ? 1 : 0};
+        const DropRate r = drop_rate(da, b);
+        o.k0 = r.scale;
+        o.k1 = __uint_as_float(r.hi);
+        o.k2 = __uint_as_float(r.lo);
+        o.k3 = __uint_as_float(r.k0);
+        o.k4 = __uint_as_float(r.k1);
+        o.h0 = r.e_lo;
+        o.h1 = r.e_hi;
+        // channelwise: the whole channel's keep word
+        o.h2 = (op.flags & BA_DROPOUT_CHANNEL) && drop_keep_channel(r, c) ? 0xFFFFFFFFu : 0u;
+      }
+      break;
     default:
       break;
   }
@@ -474,6 +505,22 @@ __device__ __forceinline__ void apply_one(const ChainArgs& a, int oi, const OpCo
         }
         break;
       }
+      case BA_OP_DROPOUT:
+        if constexpr (KIND == BA_OP_DROPOUT || KIND == -2) {
+          if (!on) break;
+          // VEC divides s0; values s0 .. are numbers s0 % 8 .. of their block
+          const uint32_t w = (op.flags & BA_DROPOUT_CHANNEL)
+                                 ? k.h2
+                                 : drop_keep(drop_of(k), (uint64_t)(c * ((a.HWD + 7) >> 3) +
+                                                                    (s0 >> 3)));
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int j = (int)(s0 & 7) + i;
+            const uint32_t stays = (w << (j >> 1)) & (j & 1 ? 0x80000000u : 0x8000u);
+            v[i] = stays ? round_dt<DT>(v[i] * k.k0) : 0.0f;
+          }
+        }
+        break;
       default:
         break;
     }
@@ -482,7 +529,8 @@ __device__ __forceinline__ void apply_one(const ChainArgs& a, int oi, const OpCo
 
 // The segment's ops, in order, on n consecutive values of one channel.
 // SEQ >= 0: the ops' kinds in compile-time form, four bits each, the first
-// op in the lowest bits (0 ends the sequence); -1: any ops.
+// op in the lowest bits (0 ends the sequence); -1: any ops but a dropout, -2:
+// any ops.
 template <int DT, int VEC, int SEQ>
 __device__ __forceinline__ void apply_seq(const ChainArgs& a, const OpConst* oc, int oi,
                                           int64_t b, int64_t c, int64_t s0, int n, float* v) {
@@ -498,7 +546,7 @@ __device__ __forceinline__ void apply_ops(const ChainArgs& a, const OpConst* oc,
   if constexpr (SEQ >= 0)
     apply_seq<DT, VEC, SEQ>(a, oc, 0, b, c, s0, n, v);
   else
-    for (int oi = 0; oi < a.n_ops; ++oi) apply_one<DT, VEC>(a, oi, oc[oi], b, c, s0, n, v);
+    for (int oi = 0; oi < a.n_ops; ++oi) apply_one<DT, VEC, SEQ>(a, oi, oc[oi], b, c, s0, n, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -665,7 +713,7 @@ __device__ __forceinline__ void apply_ops_bf16x8(const ChainArgs& a, const OpCon
   if constexpr (SEQ >= 0)
     apply_seq_bf16x8<SEQ>(a, oc, 0, b, c, s0, w);
   else
-    for (int oi = 0; oi < a.n_ops; ++oi) apply_one_bf16x8<-1>(a, oi, oc[oi], b, c, s0, w);
+    for (int oi = 0; oi < a.n_ops; ++oi) apply_one_bf16x8<SEQ>(a, oi, oc[oi], b, c, s0, w);
 }
 
 __device__ __forceinline__ void fold_minmax_bf16x8(const uint32_t* w, __nv_bfloat162& mn,
@@ -880,7 +928,7 @@ __device__ __forceinline__ void run_range_vec(const ChainArgs& a, const OpConst*
 
 // Scalar path (spatial size not a multiple of the vector width, or
 // unaligned pointers): one element at a time.
-template <int DT, bool WRITE>
+template <int DT, bool WRITE, int SEQ>
 __device__ __forceinline__ void run_range_scalar(const ChainArgs& a, const OpConst* oc,
                                                  int64_t b, int64_t c, int64_t s_begin,
                                                  int64_t s_end, bool stats, float& mn, float& mx,
@@ -889,7 +937,7 @@ __device__ __forceinline__ void run_range_scalar(const ChainArgs& a, const OpCon
   for (int64_t s = s_begin + threadIdx.x; s < s_end; s += CHAIN_THREADS) {
     float v[1];
     v[0] = load_f(a.src, DT, base + s);
-    apply_ops<DT, 1>(a, oc, b, c, s, 1, v);
+    apply_ops<DT, 1, SEQ>(a, oc, b, c, s, 1, v);
     if (WRITE) store_f(a.dst, DT, base + s, v[0]);
     if (stats) {
       if (a.stats_moments)
@@ -905,7 +953,7 @@ __device__ __forceinline__ void run_range_scalar(const ChainArgs& a, const OpCon
 // ring runs uninterrupted over the whole range and the op constants are
 // resolved once per CTA.  SEQ >= 0: the segment's op kinds, four bits each
 // (first op lowest), so their dispatch is resolved at compile time; -1: any
-// ops.
+// ops but a dropout; -2: any ops.
 template <int DT, int VEC, bool WRITE, int SEQ = -1>
 __global__ void __launch_bounds__(CHAIN_THREADS, chain_minblocks<DT>())
     chain_kernel(const __grid_constant__ ChainArgs a) {
@@ -915,7 +963,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, chain_minblocks<DT>())
   const int64_t c = blockIdx.y % a.C;
   const int64_t s_begin = (int64_t)blockIdx.x * a.tile;
   const int64_t s_end = min(s_begin + a.tile, a.HWD);
-  if (threadIdx.x < a.n_ops) resolve_op<DT>(a, threadIdx.x, b, c, s_oc[threadIdx.x]);
+  if (threadIdx.x < a.n_ops)
+    resolve_op<DT, SEQ == -2 || SEQ == BA_OP_DROPOUT>(a, threadIdx.x, b, c, s_oc[threadIdx.x]);
   __syncthreads();
   float mn = INFINITY, mx = -INFINITY;
   Moments mo = {0.0, 0.0, 0.0};
@@ -923,7 +972,7 @@ __global__ void __launch_bounds__(CHAIN_THREADS, chain_minblocks<DT>())
     run_range_vec<DT, VEC, WRITE, SEQ>(a, s_oc, b, c, s_begin, s_end, a.stats_mode != 0, mn, mx,
                                        mo, s_ring);
   else
-    run_range_scalar<DT, WRITE>(a, s_oc, b, c, s_begin, s_end, a.stats_mode != 0, mn, mx, mo);
+    run_range_scalar<DT, WRITE, SEQ>(a, s_oc, b, c, s_begin, s_end, a.stats_mode != 0, mn, mx, mo);
   if (a.stats_mode != 0) {
     const int64_t g = a.stats_mode == 2 ? b * a.C + c : b;
     if (a.stats_moments)
@@ -1123,6 +1172,7 @@ ba_status launch_segment(ChainArgs& a, int64_t nb, bool write, cudaStream_t st) 
         BA_SEQ(BA_OP_RICIAN)
         BA_SEQ(BA_OP_STD_SHIFT)
         BA_SEQ(BA_OP_FIXED_MEAN)
+        BA_SEQ(BA_OP_DROPOUT)
         BA_SEQ(BA_OP_CONTRAST | BA_OP_SCALE << 4 | BA_OP_SHIFT << 8)
 #undef BA_SEQ
         default:
@@ -1134,7 +1184,11 @@ ba_status launch_segment(ChainArgs& a, int64_t nb, bool write, cudaStream_t st) 
       return check_launch("ba_intensity_chain");
     }
   }
-  if (write)
+  bool drop = false;
+  for (int i = 0; i < a.n_ops; ++i) drop = drop || a.ops[i].kind == BA_OP_DROPOUT;
+  if (drop)  // a segment with ops is written
+    chain_kernel<DT, VEC, true, -2><<<grid, CHAIN_THREADS, 0, st>>>(a);
+  else if (write)
     chain_kernel<DT, VEC, true><<<grid, CHAIN_THREADS, 0, st>>>(a);
   else
     chain_kernel<DT, VEC, false><<<grid, CHAIN_THREADS, 0, st>>>(a);
@@ -1188,7 +1242,7 @@ ba_status validate_chain(const ba_chain_desc* d) {
              d->n_ops, BA_MAX_OPS);
   for (int i = 0; i < d->n_ops; ++i) {
     const ba_op& op = d->ops[i];
-    BA_REQUIRE(op.kind >= BA_OP_NOISE && op.kind <= BA_OP_FIXED_MEAN,
+    BA_REQUIRE(op.kind >= BA_OP_NOISE && op.kind <= BA_OP_DROPOUT,
                "ba_intensity_chain: op %d unknown kind %d", i, op.kind);
     switch (op.kind) {
       case BA_OP_NOISE:
@@ -1213,6 +1267,11 @@ ba_status validate_chain(const ba_chain_desc* d) {
       case BA_OP_STD_SHIFT:
       case BA_OP_FIXED_MEAN:
         BA_REQUIRE(op.param, "ba_intensity_chain: op %d needs its per-element factor", i);
+        break;
+      case BA_OP_DROPOUT:
+        BA_REQUIRE(op.param, "ba_intensity_chain: op %d DROPOUT needs its per-element rate", i);
+        BA_REQUIRE((op.flags & ~(BA_DROPOUT_CHANNEL | BA_DROPOUT_RESCALE)) == 0,
+                   "ba_intensity_chain: op %d DROPOUT has unknown flags 0x%x", i, op.flags);
         break;
       case BA_OP_RESCALE:
         if (op.flags & BA_RESCALE_GIVEN)

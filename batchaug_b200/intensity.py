@@ -2,7 +2,8 @@
 RandAdjustContrast, RandScaleIntensity, RandShiftIntensity,
 RandStdShiftIntensity, RandScaleIntensityFixedMean, RandBiasField,
 ScaleIntensity, RandGaussianSmooth, RandGaussianSharpen,
-RandSimulateLowResolution (+ dict wrappers).
+RandSimulateLowResolution (+ dict wrappers), and two transforms the
+reference does not have: RandVoxelDropout and NormalizeIntensity.
 
 Constructors, params keys and results follow the reference PyTorch backend
 (batchaug/pytorch/intensity/*.py), op by op in the tensor dtype.  Each
@@ -389,6 +390,68 @@ class ScaleIntensity(_FusibleIntensity):
         return super().apply(tensor, params)
 
 
+class RandVoxelDropout(_FusibleIntensity):
+    """Zero each voxel of a selected element with a probability ~ U(rate) of
+    its own (a number: that probability); ``channel_wise`` zeroes whole
+    channels instead, and ``rescale`` scales what stays by 1 / (1 - rate).
+
+    No counterpart in the reference.  The mask is drawn in-kernel from the
+    params' ``drop_seed`` (``ops.dropout``: keyed on the global element, the
+    channel and the voxel) and never stored."""
+
+    _stream = _rng.S_DROPOUT
+
+    def __init__(self, prob: float = 0.1, rate=(0.0, 0.2), channel_wise: bool = False,
+                 rescale: bool = False):
+        super().__init__(prob=prob)
+        lo, hi = (rate, rate) if isinstance(rate, (int, float)) else rate
+        if not 0.0 <= lo <= hi <= 1.0:
+            raise ValueError(f"rate must lie in [0, 1], got {rate}")
+        self.rate = (float(lo), float(hi))
+        self.channel_wise = channel_wise
+        self.rescale = rescale
+
+    def _n_uniforms(self, shape):
+        return 2
+
+    def _host_params(self, B, shape, u, seed):
+        lo, hi = self.rate
+        return {"mask": u[:, 0] < self.prob,
+                "rate": (u[:, 1] * np.float32(hi - lo) + np.float32(lo)).astype(np.float32),
+                "drop_seed": seed}
+
+    def _device_params(self, host, shape, device):
+        p = upload({"mask": host["mask"], "rate": host["rate"]}, device)
+        p["drop_seed"] = host["drop_seed"]
+        p["elem_offset"] = _rng.element_offset()
+        return p
+
+    def chain_op(self, params, tensor):
+        dev = tensor.device
+        flags = (L.BA_DROPOUT_CHANNEL if self.channel_wise else 0) | \
+            (L.BA_DROPOUT_RESCALE if self.rescale else 0)
+        return ops.ChainOp(L.BA_OP_DROPOUT, flags=flags, mask=_mask_u8(params, dev),
+                           param=_dev(params, "rate", dev).to(torch.float32).contiguous(),
+                           seed=params["drop_seed"], elem_offset=params.get("elem_offset", 0))
+
+
+class NormalizeIntensity(BatchTransform):
+    """(x - mean) / sqrt(var + eps) of each channel of an element, or of the
+    whole element (``channel_wise=False``): ``ops.group_norm`` without affine
+    or activation, in fp32 with one rounding to the tensor's type.
+    Differentiable, and takes channels-last tensors as they are.  No
+    counterpart in the reference, whose ScaleIntensity goes by minimum and
+    maximum."""
+
+    def __init__(self, channel_wise: bool = True, eps: float = 1e-5):
+        super().__init__(prob=1.0)
+        self.channel_wise = channel_wise
+        self.eps = eps
+
+    def apply(self, tensor, params):
+        return ops.group_norm(tensor, tensor.shape[1] if self.channel_wise else 1, eps=self.eps)
+
+
 class RandGaussianSmooth(BatchTransform):
     """Separable Gaussian blur with per-element, per-axis sigma
     (smooth.py:91-143)."""
@@ -592,6 +655,21 @@ class ScaleIntensityd(BatchDictTransform):
     def __init__(self, keys, minv=0.0, maxv=1.0, factor=None, channel_wise: bool = True):
         super().__init__(keys=keys, transform=ScaleIntensity(minv=minv, maxv=maxv, factor=factor,
                                                              channel_wise=channel_wise))
+
+
+class RandVoxelDropoutd(BatchDictTransform):
+    """Every key gets the same draws: a channel has the same mask in each."""
+
+    def __init__(self, keys, prob: float = 0.1, rate=(0.0, 0.2), channel_wise: bool = False,
+                 rescale: bool = False):
+        super().__init__(keys=keys, transform=RandVoxelDropout(
+            prob=prob, rate=rate, channel_wise=channel_wise, rescale=rescale))
+
+
+class NormalizeIntensityd(BatchDictTransform):
+    def __init__(self, keys, channel_wise: bool = True, eps: float = 1e-5):
+        super().__init__(keys=keys, transform=NormalizeIntensity(channel_wise=channel_wise,
+                                                                 eps=eps))
 
 
 class RandGaussianSmoothd(BatchDictTransform):

@@ -156,7 +156,8 @@ typedef enum ba_op_kind {
   BA_OP_RESCALE = 6,    /* ScaleIntensity min/max rescale  contrast.py:35-68 */
   BA_OP_RICIAN = 7,     /* sqrt((x+n1)^2 + n2^2)           noise.py:146-164 */
   BA_OP_STD_SHIFT = 8,  /* x + factor * std(x)             scale_shift.py:168-198 */
-  BA_OP_FIXED_MEAN = 9  /* mean + (x - mean) * (1+factor)  scale_shift.py:252-274 */
+  BA_OP_FIXED_MEAN = 9, /* mean + (x - mean) * (1+factor)  scale_shift.py:252-274 */
+  BA_OP_DROPOUT = 10    /* ba_dropout of the selected elements (flags: BA_DROPOUT_*) */
 } ba_op_kind;
 
 /* ba_op.flags */
@@ -183,13 +184,14 @@ typedef struct ba_op {
   const uint8_t* mask; /* (B,) 0/1 or NULL = every element (RESCALE ignores it) */
   const float* param;  /* NOISE: std (B,); CONTRAST: gamma (B,); SCALE: factor (B,);
                           SHIFT: offset (B,); BIAS_FIELD: coeffs (B, n_coeff);
-                          RICIAN: noise_std (B,); STD_SHIFT, FIXED_MEAN: factor (B,) */
+                          RICIAN: noise_std (B,); STD_SHIFT, FIXED_MEAN: factor (B,);
+                          DROPOUT: rate (B,) */
   const float* param2; /* NOISE: mean (B,); RICIAN without BA_RICIAN_PHILOX:
                           injected u2, fp32 (B,C,H,W,D) */
   const float* noise;  /* NOISE without BA_NOISE_PHILOX: injected noise, fp32
                           (B,C,H,W,D), already scaled by std and shifted by mean;
                           RICIAN without BA_RICIAN_PHILOX: injected u1 */
-  uint64_t seed;        /* NOISE / RICIAN with the Philox flag: Philox key */
+  uint64_t seed;        /* NOISE / RICIAN with the Philox flag, DROPOUT: Philox key */
   uint64_t elem_offset; /* ... and the global index of element 0 */
   int32_t degree;       /* BIAS_FIELD: Legendre degree 1..6 */
   int32_t reserved;

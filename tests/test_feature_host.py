@@ -123,3 +123,38 @@ def test_reference_bits_known_answer():
     assert [int(v) for v in w] == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
     r = R.numbers(2, 3, 1000, 5)
     assert abs(r.mean() / 2**32 - 0.5) < 0.02 and len(np.unique(r)) == r.size
+
+
+def test_dropout_op_of_a_chain(ba):
+    from batchaug_b200 import _lib as L
+    c = L.ChainDesc()
+    c.batch, c.channels, c.H, c.W, c.D, c.dtype, c.n_ops = 1, 1, 2, 2, 2, 0, 1
+    c.ops[0].kind = L.BA_OP_DROPOUT
+    assert L.lib.ba_intensity_chain(ctypes.byref(c), None, 0, None) == L.BA_EINVAL
+    assert b"rate" in L.lib.ba_last_error()
+    c.ops[0].param, c.ops[0].flags = 8, 4
+    assert L.lib.ba_intensity_chain(ctypes.byref(c), None, 0, None) == L.BA_EINVAL
+    assert b"flags" in L.lib.ba_last_error()
+    c.ops[0].kind = L.BA_OP_DROPOUT + 1
+    assert L.lib.ba_intensity_chain(ctypes.byref(c), None, 0, None) == L.BA_EINVAL
+    assert b"unknown kind" in L.lib.ba_last_error()
+
+
+def test_transform_params_on_the_host(ba):
+    """The dropout transform's draws are keyed on the global element, and its
+    chain op carries seed, offset and flags."""
+    from batchaug_b200 import _lib as L
+    t = ba.RandVoxelDropout(prob=0.5, rate=(0.1, 0.3), channel_wise=True)
+    torch.manual_seed(1)
+    whole = t.sample_host(6, (6, 2, 4, 4, 4))
+    torch.manual_seed(1)
+    with ba.shard(4, 6):
+        p = t.sample_params(2, (2, 2, 4, 4, 4), torch.device("cpu"))
+    part = p["_host"]
+    assert np.array_equal(whole["mask"][4:], part["mask"])
+    assert np.array_equal(whole["rate"][4:], part["rate"]) and whole["drop_seed"] == p["drop_seed"]
+    assert ((whole["rate"] >= 0.1) & (whole["rate"] < 0.3)).all()
+    op = t.chain_op(p, torch.zeros(2, 2, 4, 4, 4))
+    assert op.kind == L.BA_OP_DROPOUT and op.flags == L.BA_DROPOUT_CHANNEL
+    assert op.seed == p["drop_seed"] and op.elem_offset == 4
+    assert ba.NormalizeIntensityd(["x"], channel_wise=False).transform.channel_wise is False
