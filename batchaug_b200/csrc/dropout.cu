@@ -14,7 +14,7 @@ struct DropoutArgs {
 };
 
 // 8 rows of the thread's columns a pass, each channel's bits from one block.
-template <int DT, int VEC>
+template <int DT, int VEC, int KEYS>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_last(const __grid_constant__ DropoutArgs a) {
   const uint32_t b = blockIdx.x / a.f.nchunk;
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(FEAT_THREADS)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (r + j < p.rows) x[j] = raw_load<DT, VEC>(src + row_at(r + j, row));
-    if (!a.channelwise) last_keep<VEC>(a.f, dr, p, r, keep);
+    if (!a.channelwise) last_keep<VEC, KEYS>(a.f, a.drop, dr, p, r, keep);
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(FEAT_THREADS)
   }
 }
 
-template <int DT, int VEC>
+template <int DT, int VEC, int KEYS>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_first(const __grid_constant__ DropoutArgs a) {
   FirstPlace p;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(FEAT_THREADS)
 #pragma unroll
           for (int i = 0; i < 8 / VEC; ++i) keep[i] = row;
         } else {
-          first_keep<VEC>(a.f, dr, p, su, keep);
+          first_keep<VEC, KEYS>(a.f, a.drop, dr, p, su, keep);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -99,12 +99,20 @@ __global__ void __launch_bounds__(FEAT_THREADS)
   }
 }
 
+template <int DT, int VEC, int KEYS>
+void launch_keys(const DropoutArgs& a, bool last, dim3 grid, cudaStream_t st) {
+  if (last)
+    dropout_last<DT, VEC, KEYS><<<grid, FEAT_THREADS, 0, st>>>(a);
+  else if constexpr (DT == BA_F32 || VEC != 4)
+    dropout_first<DT, VEC, KEYS><<<grid, FEAT_THREADS, 0, st>>>(a);
+}
+
 template <int DT, int VEC>
 void launch(const DropoutArgs& a, bool last, dim3 grid, cudaStream_t st) {
-  if (last)
-    dropout_last<DT, VEC><<<grid, FEAT_THREADS, 0, st>>>(a);
-  else if constexpr (DT == BA_F32 || VEC != 4)
-    dropout_first<DT, VEC><<<grid, FEAT_THREADS, 0, st>>>(a);
+  if (a.drop.seed_dev == nullptr)
+    launch_keys<DT, VEC, DROP_PARAM>(a, last, grid, st);
+  else
+    launch_keys<DT, VEC, DROP_WORDS>(a, last, grid, st);
 }
 
 }  // namespace
@@ -139,6 +147,7 @@ extern "C" ba_status ba_dropout(const ba_dropout_desc* desc, ba_stream_t stream)
   a.f = feat_plan(d.batch, d.channels, S, d.dtype, d.layout, ptrs, 2);
   a.drop = {d.p, d.p_elem, d.mask, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
             d.elem_offset, (d.flags & BA_DROPOUT_RESCALE) ? 1 : 0};
+  drop_keys(a.drop);
   a.channelwise = (d.flags & BA_DROPOUT_CHANNEL) ? 1 : 0;
   dim3 grid;
   st = feat_grid("ba_dropout", a.f, d.layout, &grid);

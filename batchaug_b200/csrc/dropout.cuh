@@ -38,7 +38,20 @@ struct DropArgs {
   const uint64_t* seed_dev;  // the key in device memory, NULL: seed_lo / seed_hi
   uint64_t elem_offset;
   int rescale;             // scale what stays by 1 / (1 - p)
+  uint32_t keys[20];       // the ten rounds' keys of seed_lo / seed_hi (drop_keys)
 };
+
+// Where a kernel has the rounds' keys from: the kernel's parameters (the
+// constant bank, an operand of the round's XOR; 18 additions of a block's 60
+// instructions less), or two words that it adds to.
+enum { DROP_NONE = 0, DROP_PARAM = 1, DROP_WORDS = 2 };
+
+inline void drop_keys(DropArgs& a) {
+  for (uint32_t i = 0; i < 10; ++i) {
+    a.keys[2 * i] = a.seed_lo + i * 0x9E3779B9u;
+    a.keys[2 * i + 1] = a.seed_hi + i * 0xBB67AE85u;
+  }
+}
 
 // An element's rate, resolved.
 struct DropRate {
@@ -72,17 +85,23 @@ __device__ __forceinline__ DropRate drop_rate(const DropArgs& a, int64_t b) {
   return r;
 }
 
-__device__ __forceinline__ U4 drop_block(const DropRate& r, uint64_t q, uint32_t stream) {
-  // philox4x32_10 with each 64-bit product as one instruction
+// philox4x32_10 with each 64-bit product as one instruction.
+template <int KEYS>
+__device__ __forceinline__ U4 drop_block(const DropArgs& a, const DropRate& r, uint64_t q,
+                                         uint32_t stream) {
   uint32_t x = (uint32_t)q, y = r.e_lo, z = r.e_hi, w = stream | (uint32_t)(q >> 32);
   uint32_t k0 = r.k0, k1 = r.k1;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
-    const uint64_t a = (uint64_t)0xD2511F53u * x, b = (uint64_t)0xCD9E8D57u * z;
-    x = (uint32_t)(b >> 32) ^ y ^ k0;
-    y = (uint32_t)b;
-    z = (uint32_t)(a >> 32) ^ w ^ k1;
-    w = (uint32_t)a;
+    const uint64_t m = (uint64_t)0xD2511F53u * x, n = (uint64_t)0xCD9E8D57u * z;
+    if constexpr (KEYS == DROP_PARAM) {
+      k0 = a.keys[2 * i];
+      k1 = a.keys[2 * i + 1];
+    }
+    x = (uint32_t)(n >> 32) ^ y ^ k0;
+    y = (uint32_t)n;
+    z = (uint32_t)(m >> 32) ^ w ^ k1;
+    w = (uint32_t)m;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
@@ -101,9 +120,11 @@ __device__ __forceinline__ uint32_t ge_halves(uint32_t a, uint32_t t) {
   return (a & ~t) | (~(a ^ t) & d);
 }
 
-static __device__ __noinline__ uint32_t drop_ties(const DropRate& r, uint64_t q, uint32_t stream_low,
-                                           const uint32_t* w, uint32_t keep) {
-  const U4 l = drop_block(r, q, stream_low);
+static __device__ __noinline__ uint32_t drop_ties(const DropRate& r, uint64_t q,
+                                                  uint32_t stream_low, U4 b, uint32_t keep) {
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+  const DropArgs none = {};
+  const U4 l = drop_block<DROP_WORDS>(none, r, q, stream_low);
   const uint32_t v[4] = {l.x, l.y, l.z, l.w};
   for (int j = 0; j < 4; ++j) {
     if ((w[j] & 0xFFFFu) == r.hi && (v[j] & 0xFFFFu) < r.lo) keep &= ~(1u << (15 - j));
@@ -112,11 +133,12 @@ static __device__ __noinline__ uint32_t drop_ties(const DropRate& r, uint64_t q,
   return keep;
 }
 
-__device__ __forceinline__ uint32_t drop_keep(const DropRate& r, uint64_t q,
+template <int KEYS>
+__device__ __forceinline__ uint32_t drop_keep(const DropArgs& a, const DropRate& r, uint64_t q,
                                               uint32_t stream = STREAM_DROP,
                                               uint32_t stream_low = STREAM_DROP_LOW) {
   if (r.hi > 0xFFFFu) return 0u;
-  const U4 b = drop_block(r, q, stream);
+  const U4 b = drop_block<KEYS>(a, r, q, stream);
   const uint32_t w[4] = {b.x, b.y, b.z, b.w};
   const uint32_t t = r.hi * 0x10001u;
   uint32_t keep = 0u;
@@ -130,14 +152,16 @@ __device__ __forceinline__ uint32_t drop_keep(const DropRate& r, uint64_t q,
       const uint32_t x = w[j] ^ t;
       tie |= (x - 0x00010001u) & ~x;
     }
-    if (tie & 0x80008000u) keep = drop_ties(r, q, stream_low, w, keep);
+    if (tie & 0x80008000u) keep = drop_ties(r, q, stream_low, b, keep);
   }
   return keep;
 }
 
 // Whether channel c of the element stays (channelwise dropout).
 __device__ __forceinline__ bool drop_keep_channel(const DropRate& r, int64_t c) {
-  const uint32_t k = drop_keep(r, (uint64_t)c >> 3, STREAM_DROP_CHANNEL, STREAM_DROP_CHANNEL_LOW);
+  const DropArgs none = {};
+  const uint32_t k = drop_keep<DROP_WORDS>(none, r, (uint64_t)c >> 3, STREAM_DROP_CHANNEL,
+                                           STREAM_DROP_CHANNEL_LOW);
   const int i = (int)(c & 7);
   return (k >> ((i & 1 ? 31 : 15) - (i >> 1))) & 1u;
 }

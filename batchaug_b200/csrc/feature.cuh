@@ -228,12 +228,12 @@ __device__ __forceinline__ uint64_t row_at(int r, uint32_t row_bytes) {
 
 // Keep words of VEC channels, for the 8 rows from row r of the item
 // (r0 + r is a multiple of 8).
-template <int VEC>
-__device__ __forceinline__ void last_keep(const Feat& f, const DropRate& dr, const LastPlace& p,
-                                          int r, uint32_t* keep) {
+template <int VEC, int KEYS>
+__device__ __forceinline__ void last_keep(const Feat& f, const DropArgs& a, const DropRate& dr,
+                                          const LastPlace& p, int r, uint32_t* keep) {
   const uint64_t q = (uint64_t)(p.c * f.nblk + ((p.r0 + r) >> 3));
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) keep[i] = drop_keep(dr, q + (uint64_t)(i * f.nblk));
+  for (int i = 0; i < VEC; ++i) keep[i] = drop_keep<KEYS>(a, dr, q + (uint64_t)(i * f.nblk));
 }
 
 // Pair i of row j (0 .. 7), its dropped elements zeroed.
@@ -323,11 +323,11 @@ __device__ __forceinline__ void first_store(char* x, int s, const FirstPlace& p,
 // draws the tile's block l, and where an access is narrower than a block the
 // words are handed over from the lanes that drew them.  k[j / VEC] belongs to
 // the values j .. j + VEC - 1, shifted so that first_pair_keep finds them.
-template <int VEC>
-__device__ __forceinline__ void first_keep(const Feat& f, const DropRate& dr, const FirstPlace& p,
-                                           int s, uint32_t* k) {
+template <int VEC, int KEYS>
+__device__ __forceinline__ void first_keep(const Feat& f, const DropArgs& a, const DropRate& dr,
+                                           const FirstPlace& p, int s, uint32_t* k) {
   const uint32_t own =
-      drop_keep(dr, (uint64_t)(p.c * f.nblk + ((p.s0 + s) >> 3) + p.lane));
+      drop_keep<KEYS>(a, dr, (uint64_t)(p.c * f.nblk + ((p.s0 + s) >> 3) + p.lane));
 #pragma unroll
   for (int j = 0; j < 8; j += VEC) {
     if constexpr (VEC == 8) {

@@ -511,8 +511,9 @@ __device__ __forceinline__ void apply_one(const ChainArgs& a, int oi, const OpCo
           // VEC divides s0; values s0 .. are numbers s0 % 8 .. of their block
           const uint32_t w = (op.flags & BA_DROPOUT_CHANNEL)
                                  ? k.h2
-                                 : drop_keep(drop_of(k), (uint64_t)(c * ((a.HWD + 7) >> 3) +
-                                                                    (s0 >> 3)));
+                                 : drop_keep<DROP_WORDS>(
+                                       DropArgs{}, drop_of(k),
+                                       (uint64_t)(c * ((a.HWD + 7) >> 3) + (s0 >> 3)));
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const int j = (int)(s0 & 7) + i;

@@ -43,7 +43,7 @@ size_t norm_smem(const NormArgs& a, bool last, int32_t dtype, bool backward) {
 // CTAs of the kernel that an SM holds; also lifts its shared memory limit.
 int norm_occupancy(NormKernel fn, const NormKind& k, int32_t dtype, int32_t layout, size_t smem) {
   // an idempotent cache: threads that fill an entry together write the same
-  static int cached[64][2][2][3][4][2][2];
+  static int cached[64][2][2][3][4][3][2];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
   int& c = cached[dev][dtype][layout][k.vec == 1 ? 0 : k.vec == 4 ? 1 : 2][k.act][k.drop]
@@ -178,7 +178,9 @@ void norm_plan(const ba_norm_desc& d, bool backward, NormCall& c) {
           : d.activation == BA_ACT_SILU ? ACT_SILU
           : d.activation == BA_ACT_GELU ? ACT_GELU
                                         : ACT_LEAKY;
-  k.drop = d.p_elem != nullptr || d.p > 0.0f;
+  k.drop = d.p_elem == nullptr && d.p <= 0.0f ? DROP_NONE
+           : d.seed_dev == nullptr            ? DROP_PARAM
+                                              : DROP_WORDS;
   k.backward = backward;
   c.fn = norm_kernel_of(k, d.dtype, d.layout);
   const bool last = d.layout == BA_CHANNELS_LAST;
@@ -256,6 +258,7 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.slope = d.activation == BA_ACT_LEAKY_RELU ? d.slope : 0.0f;
   a.drop = {d.p, d.p_elem, nullptr, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
             d.elem_offset, 1};
+  drop_keys(a.drop);
   if (cudaMemsetAsync(workspace, 0, sc.chan, cs) != cudaSuccess) {
     set_error("%s: clearing the scratch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
     return BA_ECUDA;

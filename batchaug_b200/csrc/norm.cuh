@@ -176,7 +176,7 @@ __device__ __forceinline__ PairConst pair_const(const GroupStat& g, float w, flo
 
 // x -> the results of two pairs (dy: its dropped elements zeroed); scale is
 // dropout's, 1 without it.
-template <int DT, int ACT, bool DROP, bool BWD>
+template <int DT, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void norm_pairs(RawPair<DT>& x0, RawPair<DT>& x1, RawPair<DT> d0,
                                            RawPair<DT> d1, const PairConst& k0,
                                            const PairConst& k1, float slope, float scale) {
@@ -647,12 +647,12 @@ __device__ __forceinline__ Stream<DT, VEC, BWD> last_stream(const NormArgs& a, c
 // sm: two planes of nty rows by cw channels, floats (2 * FEAT_THREADS * VEC in
 // all), or the constants; meet: max(FEAT_THREADS, cw) entries; acc: the
 // groups' sums so far and their centres.
-template <int DT, int VEC, int ACT, bool DROP, bool BWD>
+template <int DT, int VEC, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
                                           Stream<DT, VEC, BWD>& st, const char* first, uint32_t g0,
                                           const GroupStat* gs, ChanParam own, float* sm, float* wt,
                                           double2* meet, double2* acc, bool first_pass) {
-  constexpr bool BLOCK = BWD && DROP;
+  constexpr bool BLOCK = BWD && DROP != DROP_NONE;
   constexpr int NP = VEC > 1 ? VEC / 2 : 1;  // pairs of channels, or of rows
   if constexpr (BWD) st.zero(st.left);
   F2 s0[NP], s1[NP];
@@ -687,7 +687,7 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
   for (int q = 0; q < st.blocks; ++q, st.next()) {
     const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
     uint32_t keep[VEC];
-    if constexpr (BLOCK) last_keep<VEC>(a.f, dr, p, q * p.nty * 8 + p.ty * 8, keep);
+    if constexpr (BLOCK) last_keep<VEC, DROP>(a.f, a.drop, dr, p, q * p.nty * 8 + p.ty * 8, keep);
     st.fill();
     if constexpr (VEC > 1) {
 #pragma unroll
@@ -846,7 +846,7 @@ __device__ __forceinline__ void last_put(const NormArgs& a, const LastPlace& p, 
 }
 
 // y or dx of a pass of one item; the pass's first block is on its way.
-template <int DT, int VEC, int ACT, bool DROP, bool BWD>
+template <int DT, int VEC, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void last_apply(const NormArgs& a, const LastPlace& p,
                                            Stream<DT, VEC, BWD>& st, uint32_t g0,
                                            const GroupStat* gs, ChanParam own, const DropRate& dr,
@@ -865,7 +865,7 @@ __device__ __forceinline__ void last_apply(const NormArgs& a, const LastPlace& p
     const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
     uint32_t keep[VEC];
     if constexpr (DROP)
-      last_keep<VEC>(a.f, dr, p, (a.reverse ? st.blocks - 1 - q : q) * p.nty * 8 + p.ty * 8, keep);
+      last_keep<VEC, DROP>(a.f, a.drop, dr, p, (a.reverse ? st.blocks - 1 - q : q) * p.nty * 8 + p.ty * 8, keep);
     st.fill();
     if constexpr (VEC > 1) {
 #pragma unroll
@@ -954,16 +954,16 @@ __device__ __forceinline__ Stream<DT, VEC, BWD> first_stream(const NormArgs& a,
 
 // Keep words of accesses j and j + 1 of a block (k: 8 / VEC words a tile; two
 // tiles for VEC 8, one for VEC 4; a single element's tile is a block).
-template <int VEC>
+template <int VEC, int DROP>
 __device__ __forceinline__ void first_block_keep(const NormArgs& a, const DropRate& dr,
                                                  const FirstPlace& p, int s, uint32_t* k) {
-  first_keep<VEC>(a.f, dr, p, s, k);
-  if constexpr (VEC == 8) first_keep<VEC>(a.f, dr, p, s + FEAT_TILE, k + 1);
+  first_keep<VEC, DROP>(a.f, a.drop, dr, p, s, k);
+  if constexpr (VEC == 8) first_keep<VEC, DROP>(a.f, a.drop, dr, p, s + FEAT_TILE, k + 1);
 }
 
 // The partial of one item.  meet: 2 * FEAT_WARPS entries that the CTA's
 // previous call did not use.
-template <int DT, int VEC, int ACT, bool DROP, bool BWD>
+template <int DT, int VEC, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const FirstPlace& p,
                                            char* ring, double2* meet, float4* part) {
   Stream<DT, VEC, BWD> st = first_stream<DT, VEC, BWD>(a, p, ring);
@@ -995,7 +995,7 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
       for (int j = 0; j < 8; j += 2) {
         uint32_t keep[2];
         if constexpr (BWD && DROP)
-          first_block_keep<VEC>(a, dr, p, (q * 8 + j) * 32 * VEC, keep);
+          first_block_keep<VEC, DROP>(a, dr, p, (q * 8 + j) * 32 * VEC, keep);
         st.wait2();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -1020,7 +1020,7 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
       if constexpr (BWD) st.zero(more);
     } else {
       uint32_t keep[8];
-      if constexpr (BWD && DROP) first_keep<VEC>(a.f, dr, p, q * 8 * 32 * VEC, keep);
+      if constexpr (BWD && DROP) first_keep<VEC, DROP>(a.f, a.drop, dr, p, q * 8 * 32 * VEC, keep);
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {
         RawPair<DT> d[2] = {};
@@ -1090,7 +1090,7 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
   }
 }
 
-template <int DT, int VEC, int ACT, bool DROP, bool BWD>
+template <int DT, int VEC, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace& p,
                                             Stream<DT, VEC, BWD>& st, const PairConst& k,
                                             const DropRate& dr) {
@@ -1106,7 +1106,7 @@ __device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace&
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         uint32_t keep[2];
-        if constexpr (DROP) first_block_keep<VEC>(a, dr, p, s + j * 32 * VEC, keep);
+        if constexpr (DROP) first_block_keep<VEC, DROP>(a, dr, p, s + j * 32 * VEC, keep);
         st.wait2();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -1135,7 +1135,7 @@ __device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace&
       }
     } else {
       uint32_t keep[8];
-      if constexpr (DROP) first_keep<VEC>(a.f, dr, p, s, keep);
+      if constexpr (DROP) first_keep<VEC, DROP>(a.f, a.drop, dr, p, s, keep);
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {
         RawPair<DT> d[2] = {};
@@ -1198,7 +1198,7 @@ static __device__ __noinline__ void norm_param_grads(const NormArgs& a, double2*
 }
 
 // ===========================================================================
-template <int DT, bool LAST, int VEC, int ACT, bool DROP, bool BWD>
+template <int DT, bool LAST, int VEC, int ACT, int DROP, bool BWD>
 __global__ void __launch_bounds__(FEAT_THREADS, 2)
     norm_kernel(const __grid_constant__ NormArgs a) {
   // meet | group sums | group numbers | rings | weights | planes or constants
@@ -1223,7 +1223,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
         LastPlace p = last_place<VEC>(a.f, b, i, cb);
         bool first_pass = true;
         while (true) {
-          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, BWD && DROP>(a, p, ring);
+          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, (BWD && DROP != DROP_NONE)>(a, p, ring);
           const char* first = st.x;
           st.start();
           ChanParam cp = {};
@@ -1266,7 +1266,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
         if constexpr (DROP) dr = drop_rate(a.drop, p.b);
         bool first_pass = true;
         while (true) {
-          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, DROP>(a, p, ring);
+          Stream<DT, VEC, BWD> st = last_stream<DT, VEC, BWD, DROP != DROP_NONE>(a, p, ring);
           if (a.reverse) st.turn();
           st.start();
           const ChanParam cp = chan_param(a, p.c - p.tx * VEC + threadIdx.x, p.c_end);

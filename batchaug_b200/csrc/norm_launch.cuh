@@ -9,7 +9,8 @@ namespace ba {
 struct NormKind {
   int vec;
   int act;  // ACT_*
-  bool drop, backward;
+  int drop;  // DROP_*
+  bool backward;
 };
 
 using NormKernel = void (*)(NormArgs);
@@ -19,13 +20,17 @@ NormKernel norm_kernel_bf16_last(const NormKind& k);
 NormKernel norm_kernel_f32_first(const NormKind& k);
 NormKernel norm_kernel_f32_last(const NormKind& k);
 
+template <int DT, bool LAST, int VEC, int ACT, int DROP>
+NormKernel norm_kernel_drop(const NormKind& k) {
+  return k.backward ? norm_kernel<DT, LAST, VEC, ACT, DROP, true>
+                    : norm_kernel<DT, LAST, VEC, ACT, DROP, false>;
+}
+
 template <int DT, bool LAST, int VEC, int ACT>
 NormKernel norm_kernel_act(const NormKind& k) {
-  if (k.backward)
-    return k.drop ? norm_kernel<DT, LAST, VEC, ACT, true, true>
-                  : norm_kernel<DT, LAST, VEC, ACT, false, true>;
-  return k.drop ? norm_kernel<DT, LAST, VEC, ACT, true, false>
-                : norm_kernel<DT, LAST, VEC, ACT, false, false>;
+  if (k.drop == DROP_PARAM) return norm_kernel_drop<DT, LAST, VEC, ACT, DROP_PARAM>(k);
+  if (k.drop == DROP_WORDS) return norm_kernel_drop<DT, LAST, VEC, ACT, DROP_WORDS>(k);
+  return norm_kernel_drop<DT, LAST, VEC, ACT, DROP_NONE>(k);
 }
 
 template <int DT, bool LAST, int VEC>
