@@ -414,24 +414,23 @@ def _feature_map(x: torch.Tensor, name: str):
     """``x`` dense in one of the two layouts the kernels take, and which: a
     (B,C,H,W,D) tensor contiguous as named or in torch.channels_last_3d is
     taken as it is, any other strides are copied to the former."""
-    L.require_cuda(x, name)
+    if not x.is_cuda:
+        L.require_cuda(x, name)
     if x.dim() != 5:
         raise ValueError(f"expected a (B,C,H,W,D) tensor, got shape {tuple(x.shape)}")
-    if x.is_contiguous():
-        # one voxel: both layouts at once, and its channels are the long axis
-        one = x.shape[2] * x.shape[3] * x.shape[4] == 1
-        return x, L.BA_CHANNELS_LAST if one else L.BA_CHANNELS_FIRST
     if x.is_contiguous(memory_format=torch.channels_last_3d):
-        return x, L.BA_CHANNELS_LAST
-    return x.contiguous(), L.BA_CHANNELS_FIRST
+        # one channel or one voxel: both layouts at once, and what is contiguous
+        # is the longer axis
+        return x, (L.BA_CHANNELS_FIRST if x.shape[1] == 1 else L.BA_CHANNELS_LAST)
+    return (x if x.is_contiguous() else x.contiguous()), L.BA_CHANNELS_FIRST
 
 
 def _like(t: torch.Tensor, x: torch.Tensor, layout: int) -> torch.Tensor:
     """``t`` (a gradient) with x's dtype and layout."""
-    if t.dtype != x.dtype:
+    if t.dtype is not x.dtype:
         t = t.to(x.dtype)
-    return t.contiguous(memory_format=torch.channels_last_3d if layout == L.BA_CHANNELS_LAST
-                        else torch.contiguous_format)
+    f = (torch.channels_last_3d if layout == L.BA_CHANNELS_LAST else torch.contiguous_format)
+    return t if t.is_contiguous(memory_format=f) else t.contiguous(memory_format=f)
 
 
 def _drop_params(x: torch.Tensor, p, seed, name: str):
@@ -443,56 +442,60 @@ def _drop_params(x: torch.Tensor, p, seed, name: str):
             raise ValueError(f"{name}: p has {p.numel()} values for a batch of {x.shape[0]}")
         p_elem = p.detach().to(device=x.device, dtype=torch.float32).reshape(-1).contiguous()
         p = 0.0
-    else:
-        p = float(p)
-        if not 0.0 <= p <= 1.0:
-            raise ValueError(f"{name}: p={p} is not a probability")
-    if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
-            raise ValueError(f"{name}: a seed tensor must be one int64 on {x.device}")
-        seed_dev, seed = seed, 0
-    elif seed is None:
+    elif not 0.0 <= p <= 1.0:
+        raise ValueError(f"{name}: p={p} is not a probability")
+    if seed is None:
         if p_elem is not None or p > 0.0:
             raise ValueError(f"{name}: dropout needs a seed")
         seed = 0
+    elif isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+            raise ValueError(f"{name}: a seed tensor must be one int64 on {x.device}")
+        seed_dev, seed = seed, 0
     return p, p_elem, int(seed) & 0xFFFFFFFFFFFFFFFF, seed_dev
 
 
-def _launch(fn, name: str, nbytes: int, device: torch.device, *args) -> None:
-    """One C entry on the device's current stream, with the device current."""
+def _launch(fn, name: str, passes: int, x: torch.Tensor, *args) -> None:
+    """One C entry on the current stream of x's device, with that device
+    current; ``passes``: how often it moves x's bytes."""
+    device = x.device
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _launch(fn, name, nbytes, device, *args)
-    tok = _timing.begin(name, nbytes, device)
-    st = fn(*args, L.stream_ptr(device))
+            return _launch(fn, name, passes, x, *args)
+    if _timing._active is None:
+        st = fn(*args, L.stream_ptr(device))
+    else:
+        tok = _timing.begin(name, passes * x.numel() * x.element_size(), device)
+        st = fn(*args, L.stream_ptr(device))
+        _timing.end(tok)
     if st:
         L.check(st, name)
-    _timing.end(tok)
 
 
 def _dropout_call(x, desc):
     out = torch.empty_like(x)
     desc.src, desc.dst = x.data_ptr(), out.data_ptr()
-    _launch(L.lib.ba_dropout, "ba_dropout", 2 * x.numel() * x.element_size(), x.device,
-            ctypes.byref(desc))
+    _launch(L.lib.ba_dropout, "ba_dropout", 2, x, ctypes.byref(desc))
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, desc, layout, tensors):
+    def forward(ctx, x, call):
+        desc, _, tensors = ctx.call = call
         # the tensors behind the descriptor's addresses, if it has any
-        ctx.save_for_backward(*tensors)
-        ctx.desc, ctx.layout = desc, layout
+        if tensors:
+            ctx.save_for_backward(*tensors)
         return _dropout_call(x, desc)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        ctx.saved_tensors  # raises if one of them was written to since
+        desc, layout, tensors = ctx.call
+        if tensors:
+            ctx.saved_tensors  # raises if one of them was written to since
         # the same draw on the gradient
-        desc = L.DropoutDesc.from_buffer_copy(ctx.desc)
-        return _dropout_call(_like(dy, dy, ctx.layout), desc), None, None, None
+        return _dropout_call(_like(dy, dy, layout), L.DropoutDesc.from_buffer_copy(desc)), None
 
 
 def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
@@ -518,55 +521,59 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     desc = L.DropoutDesc(None, None, B, C, H, W, D, dtype, layout, flags, p, L.ptr(p_elem),
                          L.ptr(m), seed, L.ptr(seed_dev), int(elem_offset))
     if torch.is_grad_enabled() and x.requires_grad:
-        tensors = [t for t in (p_elem, m, seed_dev) if t is not None]
-        return _Dropout.apply(x, desc, layout, tensors)
+        return _Dropout.apply(x, (desc, layout,
+                                  [t for t in (p_elem, m, seed_dev) if t is not None]))
     return _dropout_call(x, desc)
 
 
-def _norm_call(fn, name, desc, backward, nbytes, device):
-    size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), backward)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _launch(fn, name, nbytes, device, ctypes.byref(desc), L.ptr(ws), size)
-
-
 def _norm_forward(x, desc, groups):
+    """y, and the buffer of the statistics (and, behind them, the scratch)."""
     y = torch.empty_like(x)
-    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
-    desc.out, desc.stats = y.data_ptr(), stats.data_ptr()
-    _norm_call(L.lib.ba_norm_forward, "ba_norm_forward", desc, 0,
-               2 * x.numel() * x.element_size(), x.device)
-    return y, stats
+    size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 0)
+    head = (x.shape[0] * groups * 8 + 15) & ~15
+    buf = torch.empty(head + size, dtype=torch.uint8, device=x.device)
+    at = buf.data_ptr()
+    desc.out, desc.stats = y.data_ptr(), at
+    _launch(L.lib.ba_norm_forward, "ba_norm_forward", 2, x, ctypes.byref(desc), at + head, size)
+    return y, buf
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, desc, groups, layout, tensors):
-        y, stats = _norm_forward(x, desc, groups)
-        ctx.desc, ctx.layout = desc, layout
+    def forward(ctx, x, weight, bias, call):
+        desc, groups, _, tensors = ctx.call = call
+        y, buf = _norm_forward(x, desc, groups)
         # x, the parameters, and what else the descriptor points to
-        ctx.save_for_backward(x, weight, bias, stats, *tensors)
+        ctx.save_for_backward(x, weight, bias, buf, *tensors)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias = ctx.saved_tensors[:3]
-        dy = _like(dy, x, ctx.layout)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty_like(bias) if need_b else None
-        desc = L.NormDesc.from_buffer_copy(ctx.desc)
-        desc.dy, desc.out = dy.data_ptr(), L.ptr(dx)
-        desc.dweight, desc.dbias = L.ptr(dw), L.ptr(db)
-        _norm_call(L.lib.ba_norm_backward, "ba_norm_backward", desc, 1,
-                   3 * x.numel() * x.element_size(), x.device)
-        return dx, dw, db, None, None, None, None
+        desc, _, layout, _ = ctx.call
+        desc = L.NormDesc.from_buffer_copy(desc)
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dy = _like(dy, x, layout)
+        dx = dw = db = None
+        desc.dy, desc.out = dy.data_ptr(), None
+        if need_x:
+            dx = torch.empty_like(x)
+            desc.out = dx.data_ptr()
+        if need_w:
+            dw = torch.empty_like(weight)
+            desc.dweight = dw.data_ptr()
+        if need_b:
+            db = torch.empty_like(bias)
+            desc.dbias = db.data_ptr()
+        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 1)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        _launch(L.lib.ba_norm_backward, "ba_norm_backward", 3, x, ctypes.byref(desc),
+                ws.data_ptr(), size)
+        return dx, dw, db, None
 
 
 def _norm_param(t, x, name):
-    if t is None:
-        return None
     if t.device != x.device:
         raise ValueError(f"group_norm: {name} is on {t.device}, x on {x.device}")
     if t.dim() != 1 or t.shape[0] != x.shape[1]:
@@ -597,12 +604,17 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     if activation not in L.ACTIVATIONS:
         raise ValueError(f"unsupported activation {activation!r} (expected one of "
                          f"{[a for a in L.ACTIVATIONS if a]})")
-    weight, bias = _norm_param(weight, x, "weight"), _norm_param(bias, x, "bias")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    param = None
+    if weight is not None:
+        param = weight = _norm_param(weight, x, "weight")
+    if bias is not None:
+        bias = _norm_param(bias, x, "bias")
+        if param is None:
+            param = bias
+        elif param.dtype is not bias.dtype:
+            raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "group_norm")
     B, C, H, W, D = x.shape
-    param = weight if weight is not None else bias
     desc = L.NormDesc(x.data_ptr(), None, None, L.ptr(weight), L.ptr(bias), None, None, None, B, C,
                       H, W, D, num_groups, dtype, layout,
                       L.BA_F32 if param is None else L.dtype_code(param),
@@ -612,7 +624,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         tensors = [t for t in (p_elem, seed_dev) if t is not None]
-        return _GroupNorm.apply(x, weight, bias, desc, num_groups, layout, tensors)
+        return _GroupNorm.apply(x, weight, bias, (desc, num_groups, layout, tensors))
     return _norm_forward(x, desc, num_groups)[0]
 
 
