@@ -15,7 +15,7 @@ struct DropoutArgs {
 
 // 8 rows of the thread's columns a pass, each channel's bits from one block.
 template <int DT, int VEC, int KEYS>
-__global__ void __launch_bounds__(FEAT_THREADS)
+__global__ void __launch_bounds__(FEAT_THREADS, 3)
     dropout_last(const __grid_constant__ DropoutArgs a) {
   const uint32_t b = blockIdx.x / a.f.nchunk;
   const LastPlace p = last_place<VEC>(a.f, b, blockIdx.x - b * a.f.nchunk, blockIdx.y);
@@ -82,17 +82,25 @@ __global__ void __launch_bounds__(FEAT_THREADS)
     for (int u = 0; u < FLIGHT; ++u) {
       const int su = s + u * FEAT_TILE;
       if (su < p.n) {
-        uint32_t keep[8 / VEC];
+        // a block of its own (four words), or handed-over keep words
+        uint32_t keep[VEC == 8 ? 4 : 8 / VEC];
         if (a.channelwise) {
 #pragma unroll
-          for (int i = 0; i < 8 / VEC; ++i) keep[i] = row;
+          for (int i = 0; i < (VEC == 8 ? 4 : 8 / VEC); ++i) keep[i] = row;
+        } else if constexpr (VEC == 8) {
+          drop_words<KEYS>(a.drop, dr,
+                           (uint64_t)(p.c * a.f.nblk + ((p.s0 + su) >> 3) + p.lane), keep);
         } else {
           first_keep<VEC, KEYS>(a.f, a.drop, dr, p, su, keep);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          t[u].p[i] = first_pair_keep<DT, VEC>(
-              pair_raw<DT>(mul2(pair_value<DT>(t[u].p[i]), scale)), keep, i);
+        for (int i = 0; i < 4; ++i) {
+          const RawPair<DT> y = pair_raw<DT>(mul2(pair_value<DT>(t[u].p[i]), scale));
+          if constexpr (VEC == 8)
+            t[u].p[i] = pair_keep<DT, 1, 3>(y, keep[i], keep[i]);
+          else
+            t[u].p[i] = first_pair_keep<DT, VEC>(y, keep, i);
+        }
         first_store<DT, VEC>(dst, su, p, t[u]);
       }
     }

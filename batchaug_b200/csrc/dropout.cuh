@@ -66,7 +66,7 @@ __device__ __forceinline__ DropRate drop_rate(const DropArgs& a, int64_t b) {
   const bool on = a.mask == nullptr || a.mask[b] != 0;
   float p = a.p_elem != nullptr ? a.p_elem[b] : a.p;
   p = (on && p > 0.0f) ? p : 0.0f;  // NaN counts as 0
-  r.scale = (a.rescale && on) ? (p < 1.0f ? __fdiv_rn(1.0f, 1.0f - p) : 0.0f) : 1.0f;
+  r.scale = (a.rescale && on) ? (p < 1.0f ? __frcp_rn(1.0f - p) : 0.0f) : 1.0f;
   // p * 2^32 is exact; below 1 it is at most 2^32 - 2^8
   const uint32_t t = p < 1.0f ? __float2uint_ru(p * 4294967296.0f) : 0u;
   r.hi = p < 1.0f ? t >> 16 : 0x10000u;
@@ -108,11 +108,6 @@ __device__ __forceinline__ U4 drop_block(const DropArgs& a, const DropRate& r, u
   return {x, y, z, w};
 }
 
-// The decisions of a block as a word K: number 2 j's is bit 15 - j, number
-// 2 j + 1's bit 31 - j (set: it stays), so that K << j has the pair's in the
-// sign bits of its halves, where one byte permutation spreads them into masks.
-constexpr uint32_t KEEP_ALL = 0xF000F000u;
-
 // Sign bits of the halves: a >= t, for two 16-bit values each.
 __device__ __forceinline__ uint32_t ge_halves(uint32_t a, uint32_t t) {
   const uint32_t h = 0x80008000u;
@@ -121,39 +116,61 @@ __device__ __forceinline__ uint32_t ge_halves(uint32_t a, uint32_t t) {
 }
 
 static __device__ __noinline__ uint32_t drop_ties(const DropRate& r, uint64_t q,
-                                                  uint32_t stream_low, U4 b, uint32_t keep) {
+                                                  uint32_t stream_low, U4 b) {
   const uint32_t w[4] = {b.x, b.y, b.z, b.w};
   const DropArgs none = {};
   const U4 l = drop_block<DROP_WORDS>(none, r, q, stream_low);
   const uint32_t v[4] = {l.x, l.y, l.z, l.w};
+  uint32_t lost = 0u;
   for (int j = 0; j < 4; ++j) {
-    if ((w[j] & 0xFFFFu) == r.hi && (v[j] & 0xFFFFu) < r.lo) keep &= ~(1u << (15 - j));
-    if ((w[j] >> 16) == r.hi && (v[j] >> 16) < r.lo) keep &= ~(1u << (31 - j));
+    if ((w[j] & 0xFFFFu) == r.hi && (v[j] & 0xFFFFu) < r.lo) lost |= 1u << (2 * j);
+    if ((w[j] >> 16) == r.hi && (v[j] >> 16) < r.lo) lost |= 2u << (2 * j);
   }
-  return keep;
+  return lost;
 }
+
+// The decisions of block q: the sign bits of the halves of g[j] say whether
+// the numbers 2 j and 2 j + 1 stay, so that one byte permutation spreads them
+// into a mask for a pair of values.
+template <int KEYS>
+__device__ __forceinline__ void drop_words(const DropArgs& a, const DropRate& r, uint64_t q,
+                                           uint32_t* g, uint32_t stream = STREAM_DROP,
+                                           uint32_t stream_low = STREAM_DROP_LOW) {
+  if (r.hi > 0xFFFFu) {
+    g[0] = g[1] = g[2] = g[3] = 0u;
+    return;
+  }
+  const U4 b = drop_block<KEYS>(a, r, q, stream);
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+  const uint32_t t = r.hi * 0x10001u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = ge_halves(w[j], t);
+  if (r.lo != 0u) {
+    // a tie is a zero half of a w ^ t, and of the least of them
+    const uint32_t x = __vminu2(__vminu2(w[0] ^ t, w[1] ^ t), __vminu2(w[2] ^ t, w[3] ^ t));
+    if ((x - 0x00010001u) & ~x & 0x80008000u) {
+      const uint32_t lost = drop_ties(r, q, stream_low, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (lost & (1u << (2 * j))) g[j] &= ~0x8000u;
+        if (lost & (2u << (2 * j))) g[j] &= ~0x80000000u;
+      }
+    }
+  }
+}
+
+// The same as one word K: number 2 j's decision is bit 15 - j, number
+// 2 j + 1's bit 31 - j, so that K << j has the pair's in the sign bits.
+constexpr uint32_t KEEP_ALL = 0xF000F000u;
 
 template <int KEYS>
 __device__ __forceinline__ uint32_t drop_keep(const DropArgs& a, const DropRate& r, uint64_t q,
                                               uint32_t stream = STREAM_DROP,
                                               uint32_t stream_low = STREAM_DROP_LOW) {
-  if (r.hi > 0xFFFFu) return 0u;
-  const U4 b = drop_block<KEYS>(a, r, q, stream);
-  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-  const uint32_t t = r.hi * 0x10001u;
-  uint32_t keep = 0u;
+  uint32_t g[4], keep = 0u;
+  drop_words<KEYS>(a, r, q, g, stream, stream_low);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) keep |= (ge_halves(w[j], t) & 0x80008000u) >> j;
-  if (r.lo != 0u) {
-    // a zero half of w ^ t: a tie
-    uint32_t tie = 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t x = w[j] ^ t;
-      tie |= (x - 0x00010001u) & ~x;
-    }
-    if (tie & 0x80008000u) keep = drop_ties(r, q, stream_low, b, keep);
-  }
+  for (int j = 0; j < 4; ++j) keep |= (g[j] & 0x80008000u) >> j;
   return keep;
 }
 

@@ -78,7 +78,10 @@ Feat feat_plan(int64_t B, int64_t C, int64_t S, int32_t dtype, int32_t layout,
     const int64_t reps = std::min<int64_t>(8, std::max<int64_t>(1, units / (device_sms() * 16)));
     f.rows = unit * reps;
   } else {
-    f.rows = (int64_t)FEAT_TILE * FEAT_RUN;
+    // 4 to 16 tiles a warp: what a warp sets up once is worth two of them
+    const int64_t tiles = (S + FEAT_TILE - 1) / FEAT_TILE * B * C;
+    const int64_t run = tiles / ((int64_t)device_sms() * 4 * FEAT_WARPS * 4);
+    f.rows = (int64_t)FEAT_TILE * std::min<int64_t>(16, std::max<int64_t>(4, run / 4 * 4));
   }
   f.nchunk = (uint32_t)((S + f.rows - 1) / f.rows);
   return f;

@@ -12,9 +12,8 @@ namespace ba {
 
 constexpr int FEAT_THREADS = 256;
 constexpr int FEAT_WARPS = FEAT_THREADS / 32;
-// channels-first: voxels of a warp tile (32 lanes x 8) and tiles of a run
+// channels-first: voxels of a warp tile (32 lanes x 8)
 constexpr int FEAT_TILE = 256;
-constexpr int FEAT_RUN = 8;
 
 struct Feat {
   int64_t B, C, S;
