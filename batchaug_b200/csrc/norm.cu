@@ -91,6 +91,19 @@ void norm_columns(NormArgs& a, int32_t dtype) {
   a.ugroups = (uint32_t)(f.width / a.Cg);
 }
 
+// The parameters' gradients after a launch of clusters, whose CTAs need not
+// all be resident and so cannot wait for each other's sums.
+template <bool LAST>
+__global__ void __launch_bounds__(FEAT_THREADS)
+    norm_param_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ double2 meet[FEAT_THREADS];
+  norm_param_grads<LAST>(a, meet);
+}
+
+// Units of at most so many bytes are clusters of up to eight CTAs.
+constexpr int64_t NORM_CLUSTER_BYTES = (int64_t)512 << 10;
+constexpr int NORM_CLUSTER = 8;
+
 // Cuts the work for `ctas` resident CTAs: waves of units, items of a unit.
 void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ctas) {
   Feat& f = a.f;
@@ -111,16 +124,31 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   a.wave = (uint32_t)wave;
   a.reverse = sets * wave * unit_bytes > NORM_L2_BYTES;
   ctas /= sets;
+  a.cluster = unit_bytes <= NORM_CLUSTER_BYTES;
+  if (a.cluster) {
+    a.sets = 1;
+    a.wave = (uint32_t)units;
+    a.reverse = 0;
+  }
   // parts of a channel's voxels, so that a wave has one item for each CTA
   const int64_t grain = last ? 8 : FEAT_TILE;  // voxels: whole dropout blocks, whole tiles
   const int64_t rows_of_unit = last ? 1 : a.Cg;
   const int64_t workers = last ? ctas : ctas * FEAT_WARPS;
   const int64_t least = last ? (int64_t)(FEAT_THREADS / f.ncw) * 8 : FEAT_TILE;
   int64_t parts = std::max<int64_t>(1, workers / (wave * rows_of_unit));
+  if (a.cluster)
+    parts = last ? NORM_CLUSTER
+                 : std::max<int64_t>(1, (int64_t)NORM_CLUSTER * FEAT_WARPS / rows_of_unit);
   parts = std::min(parts, (f.S + least - 1) / least);
   f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
   f.nchunk = (uint32_t)((f.S + f.rows - 1) / f.rows);
   a.items = (uint32_t)(last ? f.nchunk : ((int64_t)a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
+  // a group of more channels than a cluster has warps
+  if (a.cluster && a.items > NORM_CLUSTER) {
+    a.cluster = 0;
+    a.sets = (uint32_t)sets;
+    a.wave = (uint32_t)wave;
+  }
 }
 
 struct NormScratch {
@@ -259,15 +287,35 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.drop = {d.p, d.p_elem, nullptr, (uint32_t)d.seed, (uint32_t)(d.seed >> 32), d.seed_dev,
             d.elem_offset, 1};
   drop_keys(a.drop);
+  void* args[1] = {&a};
+  if (a.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = a.items;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(a.units * a.items);
+    cfg.blockDim = dim3(FEAT_THREADS);
+    cfg.dynamicSmemBytes = c.smem;
+    cfg.stream = cs;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelExC(&cfg, (const void*)c.fn, args);
+    if ((st = check_launch(what)) != BA_OK || a.chan == nullptr) return st;
+    const unsigned grid = (unsigned)std::min<int64_t>((a.f.C + 7) / 8, 65536);
+    if (d.layout == BA_CHANNELS_LAST)
+      norm_param_kernel<true><<<grid, FEAT_THREADS, 0, cs>>>(a);
+    else
+      norm_param_kernel<false><<<grid, FEAT_THREADS, 0, cs>>>(a);
+    return check_launch(what);
+  }
   if (cudaMemsetAsync(workspace, 0, sc.chan, cs) != cudaSuccess) {
     set_error("%s: clearing the scratch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
     return BA_ECUDA;
   }
   const unsigned grid =
       (unsigned)(a.sets * std::min<int64_t>(c.ctas / a.sets, (int64_t)a.wave * a.items));
-  void* args[1] = {&a};
-  cudaLaunchCooperativeKernel((const void*)c.fn, dim3(grid), dim3(FEAT_THREADS), args,
-                              c.smem, cs);
+  cudaLaunchCooperativeKernel((const void*)c.fn, dim3(grid), dim3(FEAT_THREADS), args, c.smem, cs);
   return check_launch(what);
 }
 

@@ -9,7 +9,8 @@
 //   dw_c = sum dz * xh,  db_c = sum dz   (xh = (x - mean) * rstd; over B and S)
 //   dx = rstd * (w dz - sum_g(w dz) / n - xh * sum_g(w dz xh) / n)
 //
-// One cooperative launch does it all.  A unit is what is normalised on its
+// One launch does it all, a cooperative one where a CTA waits for others that
+// are not of its cluster.  A unit is what is normalised on its
 // own: a group of an element (channels first), or the groups of a block of
 // columns of an element (channels last).  Each set of CTAs takes units in
 // waves; its CTAs share a wave's items (equal parts of its units' voxels),
@@ -21,7 +22,9 @@
 // counter, no fence, no second hop.  The sets' waves together are small
 // enough for their inputs to be in L2 still when the results read them again,
 // so HBM sees them once; where a unit alone is larger than that, the results
-// run backwards and find the end of it there.
+// run backwards and find the end of it there.  A unit that eight CTAs can hold
+// is a cluster, whose barrier takes the place of the waiting: no zeroed words
+// and no cooperative launch, which is most of what a small call costs.
 //
 // A forward partial is the first and second moment about a value near the
 // mean, that value and the count; a thread sums about its own first value, and
@@ -63,6 +66,7 @@ struct NormArgs {
   uint32_t ugroups; // groups of a unit
   uint32_t sets;    // the CTAs are so many sets, each taking every sets-th wave
   int32_t reverse; // results from the last voxel to the first
+  int32_t cluster; // a unit is a thread block cluster (small units)
   double inv_n;    // 1 / values of a group
   float eps, slope;
   DropArgs drop;
@@ -391,6 +395,12 @@ __device__ __forceinline__ bool norm_merge(const NormArgs& a, uint32_t u, bool k
     if (threadIdx.x % 32 == 0) gs[g] = group_stat<BWD>(a, at, s, m, k0, keep);
   }
   return __syncthreads_and(ok) != 0;
+}
+
+// All CTAs of the unit have written their partials.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Backward: the item's `chan` is written, and all items' are.
@@ -1163,7 +1173,7 @@ __device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace&
 // The gradients of weight and bias: 8 channels a CTA, 32 threads a channel,
 // over the chunks of every element.
 template <bool LAST>
-static __device__ __noinline__ void norm_param_grads(const NormArgs& a, double2* meet) {
+static __device__ __forceinline__ void norm_param_grads(const NormArgs& a, double2* meet) {
   const int ci = threadIdx.x % 8, part = threadIdx.x / 8;
   const int dt = a.w_bf16 ? BA_BF16 : BA_F32;
   const uint32_t n = (uint32_t)a.f.B * a.f.nchunk;
@@ -1251,10 +1261,11 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
         turn ^= 1;
       }
       if constexpr (BWD) {
-        if (a.chan != nullptr) chan_done(a);
+        if (a.chan != nullptr && !a.cluster) chan_done(a);
       }
     }
     if (a.out == nullptr) continue;
+    if (a.cluster) cluster_barrier();
     for (uint32_t t = own; t < total; t += ctas) {
       const uint32_t u = u0 + t / a.items, i = t % a.items;
       // the first block and what else the results need are on their way while
@@ -1294,7 +1305,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
     }
   }
   if constexpr (BWD) {
-    if (a.chan != nullptr) {
+    if (a.chan != nullptr && !a.cluster) {
       if (!chan_wait(a, a.units * a.items)) return;
       norm_param_grads<LAST>(a, meet);
     }
