@@ -49,17 +49,15 @@ int norm_occupancy(NormKernel fn, const NormKind& k, int32_t dtype, int32_t layo
   int& c = cached[dev][dtype][layout][k.vec == 1 ? 0 : k.vec == 4 ? 1 : 2][k.act][k.drop]
                  [k.backward];
   if (c == 0) {
-    cudaFuncAttributes at;
-    int regs = 0;
+    int held = 0;
     if (cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              NORM_MAX_SMEM) != cudaSuccess ||
-        cudaFuncGetAttributes(&at, (const void*)fn) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&regs, fn, FEAT_THREADS, 0) != cudaSuccess ||
-        regs < 1) {
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, fn, FEAT_THREADS, 0) != cudaSuccess ||
+        held < 1) {
       cudaGetLastError();
       return 1;
     }
-    c = regs;
+    c = held;
   }
   // 227 KB a CTA at most and 228 KB an SM, 1 KB of it a CTA's own
   return std::min<int>(c, std::max<int>(1, (int)(((size_t)228 << 10) / (smem + 1024))));

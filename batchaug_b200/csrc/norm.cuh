@@ -397,10 +397,11 @@ __device__ __forceinline__ bool norm_merge(const NormArgs& a, uint32_t u, bool k
   return __syncthreads_and(ok) != 0;
 }
 
-// All CTAs of the unit have written their partials.
+// All CTAs of the unit have written their partials (a warp's lanes may come
+// apart: only some of them write).
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Backward: the item's `chan` is written, and all items' are.

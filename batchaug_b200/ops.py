@@ -550,10 +550,15 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors[:3]
+        x, weight, bias, buf = ctx.saved_tensors[:4]
         desc, _, layout, _ = ctx.call
         desc = L.NormDesc.from_buffer_copy(desc)
         need_x, need_w, need_b, _ = ctx.needs_input_grad
+        # what hooks on saved tensors give back (offloading, recomputation)
+        # lies elsewhere, and may have lost its strides
+        x = _like(x, x, layout)
+        desc.x, desc.stats = x.data_ptr(), buf.data_ptr()
+        desc.weight, desc.bias = L.ptr(weight), L.ptr(bias)
         dy = _like(dy, x, layout)
         dx = dw = db = None
         desc.dy, desc.out = dy.data_ptr(), None

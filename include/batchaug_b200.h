@@ -330,7 +330,10 @@ BA_API ba_status ba_dropout(const ba_dropout_desc* desc, ba_stream_t stream);
  * not depend on timing: no sum has an order of its own.  out overlaps neither
  * x nor dy.
  * workspace: ba_norm_workspace_bytes(desc, backward) bytes of device scratch,
- * 16-byte aligned.
+ * 16-byte aligned, which no other call uses at the same time; its content
+ * does not matter.  desc: as it will be passed to the call, addresses included
+ * (the width of an access goes by them, and the cut of the work by that), on
+ * the device that it will be called on.
  */
 typedef struct ba_norm_desc {
   const void* x;  /* (B, C, H, W, D) in `layout` */
@@ -530,7 +533,8 @@ BA_API int32_t ba_version(void);
 BA_API uint64_t ba_kernel_launches(void);
 
 /* Status of the library's bounded device waits (the mbarrier waits of the
- * TMA-staged resample; each gives up after 2 s).  Synchronises `stream`,
+ * TMA-staged resample, and a group norm's for the statistics of other thread
+ * blocks; each gives up after 2 s).  Synchronises `stream`,
  * then returns BA_ETIMEOUT, and clears the record, if any wait of any
  * earlier launch on this device ran out of time (that launch's output is
  * incomplete), else BA_OK.  The only entry point that synchronises the host.

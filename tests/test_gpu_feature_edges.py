@@ -1,0 +1,163 @@
+"""Dropout and group norm where a program may take them without thinking of
+them: saved tensors that come back elsewhere, a graph walked twice, some of the
+gradients only, a first call under capture, launches side by side, offsets past
+32 bits, a great many small units.  Tolerances are test_gpu_group_norm's."""
+from __future__ import annotations
+
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+import torch.utils.checkpoint
+
+import test_gpu_group_norm as N
+
+pytestmark = pytest.mark.gpu
+
+
+def _leaves(x, kind=torch.float32):
+    w, b = N._params(x.shape[1], kind)
+    return [t.detach().clone(memory_format=torch.preserve_format).requires_grad_()
+            for t in (x, w, b)]
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_saved_tensors_that_come_back_elsewhere(ba, layout):
+    """Offloading moves what the backward pass reads, and drops its strides;
+    recomputation frees it in between."""
+    x = N._x((2, 16, 6, 7, 8), torch.float32, layout)
+    leaves = _leaves(x)
+    dy = N._x((2, 16, 6, 7, 8), torch.float32, layout, seed=1)
+
+    def run(x, w, b):  # an input of the operator's own, free once nothing saves it
+        y = ba.ops.group_norm(x * 1.0, 4, w, b, activation="silu", p=0.3, seed=5)
+        return ba.ops.dropout(y, torch.tensor([0.2, 0.4], device="cuda"), 6)
+
+    want = torch.autograd.grad(run(*leaves), leaves, dy)
+
+    def offload(pin):
+        with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+            y = run(*leaves)
+        junk = [torch.full_like(x, float("nan")) for _ in range(8)]  # over what was freed
+        got = torch.autograd.grad(y, leaves, dy)
+        del junk
+        return got
+
+    def recompute():
+        y = torch.utils.checkpoint.checkpoint(run, *leaves, use_reentrant=False)
+        junk = [torch.full_like(x, float("nan")) for _ in range(8)]
+        got = torch.autograd.grad(y, leaves, dy)
+        del junk
+        return got
+
+    for got in (offload(False), offload(True), recompute()):
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_a_graph_walked_twice_and_parts_of_it(ba):
+    x, w, b = _leaves(N._x((2, 8, 9, 10, 11), torch.bfloat16, "last"))
+    dy = N._x((2, 8, 9, 10, 11), torch.bfloat16, "last", seed=2)
+    y = ba.ops.group_norm(x, 2, w, b, activation="gelu", p=0.1, seed=1)
+    full = torch.autograd.grad(y, [x, w, b], dy, retain_graph=True)
+    again = torch.autograd.grad(y, [x, w, b], dy, retain_graph=True)
+    assert all(torch.equal(a, c) for a, c in zip(full, again))
+    # some leaves only: dx not computed, or no parameters' gradients
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+        y = ba.ops.group_norm(leaves[0], 2, *leaves[1:], activation="gelu", p=0.1, seed=1)
+        (g,) = torch.autograd.grad(y, leaves[i], dy)
+        assert torch.equal(g, full[i])
+
+
+def test_rates_of_elements_and_a_seed_on_the_device(ba):
+    x = N._x((3, 8, 5, 6, 7), torch.float32, "last")
+    rates = torch.tensor([0.0, 1.0, 0.35], device="cuda")
+    seed = torch.tensor([-3], dtype=torch.int64, device="cuda")
+    dy = N._x((3, 8, 5, 6, 7), torch.float32, "last", seed=4)
+    a, c = (x.clone(memory_format=torch.preserve_format).requires_grad_() for _ in range(2))
+    y = ba.ops.group_norm(a, 2, activation="silu", p=rates, seed=seed, elem_offset=2**32 + 5)
+    z = ba.ops.dropout(ba.ops.group_norm(c, 2, activation="silu"), rates, -3,
+                       elem_offset=2**32 + 5)
+    assert torch.equal(y, z)
+    assert not y[1].any()
+    ga, gc = torch.autograd.grad(y, a, dy)[0], torch.autograd.grad(z, c, dy)[0]
+    # dy scaled before or after one fp32 product: a few units of the terms
+    assert (ga - gc).abs().max() <= 64 * N.U * gc.abs().max()
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("shape, groups", [((5000, 16, 1, 2, 3), 4), ((700, 24, 4, 4, 4), 24)])
+def test_many_small_units(ba, shape, groups, layout):
+    N._run(ba, shape, torch.float32, layout, groups, "silu")
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_launches_side_by_side(ba, layout):
+    """Launches that fill the device and wait within themselves, from three
+    streams, with dropouts between them."""
+    from batchaug_b200 import _lib as L
+    x = N._x((2, 32, 48, 48, 48), torch.bfloat16, layout)
+    leaves = _leaves(x)
+
+    def step():
+        y = ba.ops.group_norm(leaves[0], 8, *leaves[1:], activation="silu")
+        y = ba.ops.dropout(y, 0.25, 9)
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, x))
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(8):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, c) for a, c in zip(g, want))
+    L.wait_status(x.device)
+
+
+def test_first_call_is_captured(ba):
+    """Nothing of the library has run in the process before."""
+    code = """
+import torch, batchaug_b200 as ba
+x = torch.randn(2, 16, 40, 40, 40, device='cuda')
+s = torch.randn(2, 16, 4, 4, 4, device='cuda').contiguous(memory_format=torch.channels_last_3d)
+def step():
+    return (ba.group_norm(x, 4, activation='silu', p=0.2, seed=3), ba.dropout(x, 0.5, 4),
+            ba.group_norm(s, 4), ba.group_norm(s.repeat(1, 1, 9, 9, 9), 4))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+for _ in range(2):
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, step()))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    r = subprocess.run([sys.executable, "-c", code], env=env, cwd=root, timeout=120,
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_offsets_past_32_bits(ba, layout):
+    """2.3e9 values: the last element as on its own."""
+    shape = (5, 8, 384, 384, 384)
+    fmt = torch.channels_last_3d if layout == "last" else torch.contiguous_format
+    x = torch.empty(shape, dtype=torch.bfloat16, device="cuda", memory_format=fmt).normal_()
+    tail = x[4:].clone(memory_format=torch.preserve_format)
+    y = ba.ops.dropout(x, 0.3, 8)
+    assert torch.equal(y[4:], ba.ops.dropout(tail, 0.3, 8, elem_offset=4))
+    del y
+    y = ba.ops.group_norm(x, 2)[4:].float()
+    ref = ba.ops.group_norm(tail, 2).float()
+    # either is within K (R and M below 8, rstd about 1) and a half step of the truth
+    K = 160 * N.U * 8 + 4 * N.U * 8 + 160 * N.U * 8
+    y -= ref
+    assert (y.abs_() <= 2 * K + 2 * N._half_step(torch.bfloat16) * (ref.abs_() + K)).all()
