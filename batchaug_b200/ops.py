@@ -459,7 +459,7 @@ def _launch(fn, name: str, passes: int, x: torch.Tensor, *args) -> None:
     """One C entry on the current stream of x's device, with that device
     current; ``passes``: how often it moves x's bytes."""
     device = x.device
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():  # current_device() without its checks
         with torch.cuda.device(device):
             return _launch(fn, name, passes, x, *args)
     if _timing._active is None:
@@ -470,6 +470,16 @@ def _launch(fn, name: str, passes: int, x: torch.Tensor, *args) -> None:
         _timing.end(tok)
     if st:
         L.check(st, name)
+
+
+def _once_differentiable(backward):
+    """torch's once_differentiable, whose wrapper costs a small backward pass
+    3 us, where it is not idle: while the pass itself is being recorded."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, dy):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, dy)
+    return call
 
 
 def _dropout_call(x, desc):
@@ -489,7 +499,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout_call(x, desc)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         desc, layout, tensors = ctx.call
         if tensors:
@@ -548,7 +558,7 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         x, weight, bias, buf = ctx.saved_tensors[:4]
         desc, _, layout, _ = ctx.call
