@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -109,6 +110,20 @@ class NormDesc(ctypes.Structure):
                 ("elem_offset", _U64)]
 
 
+def packed(cls):
+    """A constructor of ``cls`` from all its fields in order, addresses as
+    integers: half the time of ctypes' own for a structure of twenty (a
+    tenth of a small call)."""
+    code = {_P: "P", _I32: "i", _I64: "q", _U64: "Q", ctypes.c_float: "f"}
+    layout = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    assert layout.size == ctypes.sizeof(cls)
+    copy, pack = cls.from_buffer_copy, layout.pack
+    return lambda *fields: copy(pack(*fields))
+
+
+dropout_desc, norm_desc = packed(DropoutDesc), packed(NormDesc)
+
+
 INTERP_MODES = {"nearest": 0, "nearest-exact": 1, "trilinear": 2, "area": 3}
 
 
@@ -175,11 +190,13 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(msg)
 
 
+_DTYPES = {torch.float32: BA_F32, torch.bfloat16: BA_BF16}
+
+
 def dtype_code(t: torch.Tensor) -> int:
-    if t.dtype == torch.float32:
-        return BA_F32
-    if t.dtype == torch.bfloat16:
-        return BA_BF16
+    code = _DTYPES.get(t.dtype)
+    if code is not None:
+        return code
     raise ValueError(f"batchaug_b200 supports float32 and bfloat16 tensors, got {t.dtype}")
 
 

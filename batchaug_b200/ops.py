@@ -528,8 +528,9 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     m = _dev_mask(mask, x.shape[0], x.device)
     flags = (L.BA_DROPOUT_CHANNEL if channelwise else 0) | (L.BA_DROPOUT_RESCALE if rescale else 0)
     B, C, H, W, D = x.shape
-    desc = L.DropoutDesc(None, None, B, C, H, W, D, dtype, layout, flags, p, L.ptr(p_elem),
-                         L.ptr(m), seed, L.ptr(seed_dev), int(elem_offset))
+    desc = L.dropout_desc(0, 0, B, C, H, W, D, dtype, layout, flags, p, L.ptr(p_elem) or 0,
+                          L.ptr(m) or 0, seed, L.ptr(seed_dev) or 0,
+                          int(elem_offset) & 0xFFFFFFFFFFFFFFFF)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Dropout.apply(x, (desc, layout,
                                   [t for t in (p_elem, m, seed_dev) if t is not None]))
@@ -630,11 +631,11 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
             raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "group_norm")
     B, C, H, W, D = x.shape
-    desc = L.NormDesc(x.data_ptr(), None, None, L.ptr(weight), L.ptr(bias), None, None, None, B, C,
-                      H, W, D, num_groups, dtype, layout,
-                      L.BA_F32 if param is None else L.dtype_code(param),
-                      L.ACTIVATIONS[activation], eps, negative_slope, p, 0, L.ptr(p_elem), seed,
-                      L.ptr(seed_dev), int(elem_offset))
+    desc = L.norm_desc(x.data_ptr(), 0, 0, L.ptr(weight) or 0, L.ptr(bias) or 0, 0, 0, 0, B, C, H,
+                       W, D, num_groups, dtype, layout,
+                       L.BA_F32 if param is None else L.dtype_code(param),
+                       L.ACTIVATIONS[activation], eps, negative_slope, p, 0, L.ptr(p_elem) or 0,
+                       seed, L.ptr(seed_dev) or 0, int(elem_offset) & 0xFFFFFFFFFFFFFFFF)
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
