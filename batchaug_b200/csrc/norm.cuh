@@ -239,6 +239,14 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
+// Of N values at once, so that their shuffles and additions overlap.
+template <int N>
+__device__ __forceinline__ void warp_sums(double* v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
+}
 
 // ===========================================================================
 // Partials, from the CTA that has them to those that need them.
@@ -276,58 +284,73 @@ __device__ __forceinline__ uint4 look_part(const float4* p) {
 }
 __device__ __forceinline__ bool is_part(const uint4& t) { return t.y != 0u && t.w != 0u; }
 
-// Looks until it is there; every CTA is resident and writes its partials
-// before it reads any, so it will be, or the wait ends without it (t0: the
-// wait's begin, 0 before).
-__device__ __forceinline__ void wait_part(const NormArgs& a, const float4* p, uint4& t,
-                                          unsigned long long& t0, bool& ok) {
-  while (!is_part(t) && ok) {
-    const unsigned long long now = wall_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > NORM_WAIT_NS) {
-      note_timeout(a);
-      ok = false;
-    }
-    t = look_part(p);
-  }
-}
-
-// Sums over the partials k = first, first + step, ... of a group: forward,
-// the moments about the centre of the first one (k0); backward, the two sums.
-// False if one of them did not come.
-template <bool BWD>
-__device__ __forceinline__ bool sum_parts(const NormArgs& a, const float4* q, uint32_t first,
-                                          uint32_t step, double& s, double& m, double& k0) {
-  bool ok = true;
+// Sums over the partials k = first, first + step, ... of a group or two, whose
+// partials begin at q and, for the second (if `two`), q + next: forward, the
+// moments about the centre of the first one (k0); backward, the two sums.  A
+// look is a round trip to L2, half a microsecond and more, so NB partials of
+// each group are looked at together, and those that are missing again: every
+// CTA is resident and writes its partials before it reads any, so they will
+// come, or the wait ends without them (false).
+template <bool BWD, int GR, int NB>
+__device__ __forceinline__ bool sum_parts(const NormArgs& a, const float4* q, bool two,
+                                          int64_t next, uint32_t first, uint32_t step, double* s,
+                                          double* m, double* k0) {
   unsigned long long t0 = 0;
-  s = m = k0 = 0.0;
-  uint4 c = {};
-  if constexpr (!BWD) c = look_part(q);
-  for (uint32_t k = first; k < a.items; k += 4 * step) {
-    uint4 t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k + i * step < a.items) t[i] = look_part(q + k + i * step);
-    if constexpr (!BWD) {
-      wait_part(a, q, c, t0, ok);
-      k0 = (double)__uint_as_float(c.x);
+  for (int g = 0; g < GR; ++g) s[g] = m[g] = k0[g] = 0.0;
+#pragma unroll 1
+  for (uint32_t k = first; k < a.items; k += NB * step) {
+    // [NB]: the first partial of the group, for its centre
+    uint4 t[GR][NB + 1];
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+      for (int i = 0; i <= NB; ++i) {
+        // what does not exist is not waited for
+        const bool is = (i < NB ? k + i * step < a.items : !BWD) && (g == 0 || two);
+        t[g][i] = make_uint4(0u, is ? 0u : 1u, 0u, is ? 0u : 1u);
+      }
+    while (true) {
+      bool there = true;
+#pragma unroll
+      for (int g = 0; g < GR; ++g)
+#pragma unroll
+        for (int i = 0; i <= NB; ++i)
+          if (!is_part(t[g][i]))
+            t[g][i] = look_part(q + g * next + (i < NB ? k + i * step : 0u));
+#pragma unroll
+      for (int g = 0; g < GR; ++g)
+#pragma unroll
+        for (int i = 0; i <= NB; ++i) there = there && is_part(t[g][i]);
+      if (there) break;
+      const unsigned long long now = wall_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > NORM_WAIT_NS) {
+        note_timeout(a);
+        return false;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k + i * step < a.items) {
-        wait_part(a, q + k + i * step, t[i], t0, ok);
-        const double x = (double)__uint_as_float(t[i].x), r = (double)__uint_as_float(t[i].z);
-        if constexpr (BWD) {
-          s += x;
-          m += r;
-        } else {
-          const double n = (double)t[i].w, d = x - k0;
-          s += n * d + r;
-          m += (double)__uint_as_float(t[i].y & 0x7FFFFFFFu) + d * (2.0 * r + n * d);
+    for (int g = 0; g < GR; ++g) {
+      if constexpr (!BWD) k0[g] = (double)__uint_as_float(t[g][NB].x);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint4& v = t[g][i];
+        if (k + i * step < a.items) {
+          const double x = (double)__uint_as_float(v.x), r = (double)__uint_as_float(v.z);
+          if constexpr (BWD) {
+            s[g] += x;
+            m[g] += r;
+          } else {
+            const double n = (double)v.w, d = x - k0[g], nd = n * d;
+            s[g] += nd + r;
+            m[g] += (double)__uint_as_float(v.y & 0x7FFFFFFFu) + d * (2.0 * r + nd);
+          }
         }
       }
+    }
   }
-  return ok;
+  return true;
 }
 
 // A group's partial from sums about k0 (forward), n values.
@@ -360,17 +383,17 @@ __device__ __forceinline__ GroupStat group_stat(const NormArgs& a, int64_t at, d
 template <bool BWD>
 __device__ __forceinline__ bool norm_merge_one(const NormArgs& a, uint32_t u, bool keep,
                                                double2* meet, GroupStat& r) {
-  double s, m, k0;
-  bool ok = sum_parts<BWD>(a, a.part + (int64_t)u * a.items, threadIdx.x, FEAT_THREADS, s, m, k0);
+  double v[2], k0;
+  bool ok = sum_parts<BWD, 1, 2>(a, a.part + (int64_t)u * a.items, false, 0, threadIdx.x,
+                                 FEAT_THREADS, v, v + 1, &k0);
   // a thread without a partial of its own has not seen the centre
-  s = warp_sum(s);
-  m = warp_sum(m);
+  warp_sums<2>(v);
   if (threadIdx.x % 32 == 0) {
-    meet[threadIdx.x / 32] = make_double2(s, m);
+    meet[threadIdx.x / 32] = make_double2(v[0], v[1]);
     if (threadIdx.x == 0) meet[FEAT_WARPS].x = k0;
   }
   ok = __syncthreads_and(ok);
-  s = m = 0.0;
+  double s = 0.0, m = 0.0;
 #pragma unroll
   for (int i = 0; i < FEAT_WARPS; ++i) {
     s += meet[i].x;
@@ -380,19 +403,26 @@ __device__ __forceinline__ bool norm_merge_one(const NormArgs& a, uint32_t u, bo
   return ok;
 }
 
-// The numbers of the unit's groups in shared memory, a warp a group.
+// The numbers of the unit's groups in shared memory, a warp two groups at a
+// time; five partials a lane are one from every SM.
 template <bool BWD>
 __device__ __forceinline__ bool norm_merge(const NormArgs& a, uint32_t u, bool keep,
                                            GroupStat* gs) {
   bool ok = true;
+  const int lane = threadIdx.x % 32;
 #pragma unroll 1
-  for (uint32_t g = threadIdx.x / 32; g < a.ugroups; g += FEAT_WARPS) {
+  for (uint32_t g = threadIdx.x / 32; g < a.ugroups; g += 2 * FEAT_WARPS) {
     const int64_t at = (int64_t)u * a.ugroups + g;
-    double s, m, k0;
-    ok = sum_parts<BWD>(a, a.part + at * a.items, threadIdx.x % 32, 32, s, m, k0) && ok;
-    s = warp_sum(s);
-    m = warp_sum(m);
-    if (threadIdx.x % 32 == 0) gs[g] = group_stat<BWD>(a, at, s, m, k0, keep);
+    const bool two = g + FEAT_WARPS < a.ugroups;
+    double v[4], k0[2];
+    ok = sum_parts<BWD, 2, 5>(a, a.part + at * a.items, two, (int64_t)FEAT_WARPS * a.items, lane,
+                              32, v, v + 2, k0) && ok;
+    warp_sums<4>(v);
+    // lane 0 has the centres
+    if (lane == 0) {
+      gs[g] = group_stat<BWD>(a, at, v[0], v[2], k0[0], keep);
+      if (two) gs[g + FEAT_WARPS] = group_stat<BWD>(a, at + FEAT_WARPS, v[1], v[3], k0[1], keep);
+    }
   }
   return __syncthreads_and(ok) != 0;
 }
@@ -662,7 +692,7 @@ template <int DT, int VEC, int ACT, int DROP, bool BWD>
 __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
                                           Stream<DT, VEC, BWD>& st, const char* first, uint32_t g0,
                                           const GroupStat* gs, ChanParam own, float* sm, float* wt,
-                                          double2* meet, double2* acc, bool first_pass) {
+                                          double2* meet, double2* acc) {
   constexpr bool BLOCK = BWD && DROP != DROP_NONE;
   constexpr int NP = VEC > 1 ? VEC / 2 : 1;  // pairs of channels, or of rows
   if constexpr (BWD) st.zero(st.left);
@@ -747,6 +777,7 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
   const float inv = 1.0f / (float)(n0 + (p.ty < y1 ? 1 : 0));
   __syncthreads();
   if (p.ty < p.nty) {
+    float us[VEC], ws[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int h = VEC > 1 ? i / 2 : 0;
@@ -758,72 +789,94 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
         u = m - (i & 1 ? k[h].nmean.y() : k[h].nmean.x());
         w = __fmaf_rn(-t, m, w);
       }
-      sm[p.ty * cw + p.tx * VEC + i] = u;
-      plane[p.ty * cw + p.tx * VEC + i] = w;
+      us[i] = u;
+      ws[i] = w;
+    }
+    const int at = p.ty * cw + p.tx * VEC;
+    if constexpr (VEC > 1) {  // wide, or eight lanes meet in a bank
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        *reinterpret_cast<float4*>(sm + at + i) = make_float4(us[i], us[i + 1], us[i + 2], us[i + 3]);
+        *reinterpret_cast<float4*>(plane + at + i) =
+            make_float4(ws[i], ws[i + 1], ws[i + 2], ws[i + 3]);
+      }
+    } else {
+      sm[at] = us[0];
+      plane[at] = ws[0];
     }
   }
   __syncthreads();
   // rows -> channel parts, about the mean of the group's first channel's first
-  // row; then, a warp a group, -> groups
+  // row (VEC rows at most, so in fp32: a conversion costs as much as four
+  // additions); then, a warp a group, -> groups, in double
   const int parts = cw >= FEAT_THREADS ? 1 : FEAT_THREADS / cw;
   const int64_t c0 = p.c - p.tx * VEC;
   const int nch = (int)min((int64_t)cw, p.c_end - c0);  // channels of the pass
+  const uint32_t ga = (uint32_t)c0 / a.Cg, gb = (uint32_t)(c0 + nch - 1) / a.Cg;
+  const float rows0 = (float)n0, rows1 = (float)(n0 + 1);
 #pragma unroll 1
   for (int cb = 0; cb < cw; cb += FEAT_THREADS) {
-    const int ci = cb + (parts == 1 ? (int)threadIdx.x : (int)threadIdx.x % cw);
-    const int part = parts == 1 ? 0 : threadIdx.x / cw;
+    const int part = parts == 1 ? 0 : (int)threadIdx.x / cw;
+    const int ci = cb + (int)threadIdx.x - part * cw;
     if (part >= parts || ci >= nch) continue;
-    double u = 0.0, w = 0.0, k0 = 0.0;
+    float u = 0.0f, w = 0.0f, k0 = 0.0f;
     const uint32_t g = (uint32_t)(c0 + ci) / a.Cg;
-    if constexpr (!BWD) {
-      const int i0 = (int)max((int64_t)0, (int64_t)g * a.Cg - c0);
-      k0 = first_pass ? (double)sm[i0] : acc[2 * (g - g0) + 1].x;
-    }
-#pragma unroll 2
+    // about the first channel of the group, which an earlier pass may have had
+    if constexpr (!BWD)
+      k0 = g * a.Cg >= (uint32_t)c0 ? sm[g * a.Cg - (uint32_t)c0] : (float)acc[2 * (g - g0) + 1].x;
+#pragma unroll 4
     for (int y = part; y < p.nty && (BWD || y < rows); y += parts) {
       const float q = sm[y * cw + ci], m2 = plane[y * cw + ci];
       if constexpr (BWD) {
-        u += (double)q;
-        w += (double)m2;
+        u += q;
+        w += m2;
       } else {
-        const double n = (double)(n0 + (y < y1 ? 1 : 0)), d = (double)q - k0;
-        u += n * d;
-        w += (double)m2 + n * d * d;
+        const float d = q - k0, nd = (y < y1 ? rows1 : rows0) * d;
+        u += nd;
+        w += __fmaf_rn(nd, d, m2);
       }
     }
+    double2 t = make_double2((double)u, (double)w);
     if constexpr (BWD) {
       const double sc = DROP ? (double)dr.scale : 1.0;
-      u *= sc;
-      w *= sc * (double)gs[g - g0].rstd;
+      t.x *= sc;
+      t.y *= sc * (double)gs[g - g0].rstd;
     }
-    meet[part * cw + ci] = make_double2(u, w);
+    meet[part * cw + ci] = t;
   }
   __syncthreads();
-  const uint32_t ga = (uint32_t)c0 / a.Cg, gb = (uint32_t)(c0 + nch - 1) / a.Cg;
   // a group is always the same warp's, so its sums are too
 #pragma unroll 1
-  for (uint32_t g = threadIdx.x / 32 + g0; g <= gb; g += FEAT_WARPS) {
-    if (g < ga) continue;
-    const int i0 = (int)max((int64_t)0, (int64_t)g * a.Cg - c0);
-    const int ng = (int)min((int64_t)nch, (int64_t)(g + 1) * a.Cg - c0) - i0;
-    double u = 0.0, w = 0.0;
-    for (int e = threadIdx.x % 32; e < ng * parts; e += 32) {
-      const int part = e / ng, i = i0 + e - part * ng;
-      const double2 t = meet[part * cw + i];
-      const double f = BWD ? (double)wt[i] : 1.0;
-      u += f * t.x;
-      w += f * t.y;
+  for (uint32_t g = threadIdx.x / 32 + g0; g <= gb; g += 2 * FEAT_WARPS) {
+    double v[4] = {0.0, 0.0, 0.0, 0.0};  // two groups' sums, then their second ones
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t gh = g + h * FEAT_WARPS;
+      if (gh < ga || gh > gb) continue;
+      const int i0 = gh > ga ? (int)(gh * a.Cg - (uint32_t)c0) : 0;
+      const int ng = (int)min((int64_t)nch, (int64_t)(gh + 1) * a.Cg - c0) - i0;
+      for (int e = threadIdx.x % 32; e < ng * parts; e += 32) {
+        const int part = e / ng, i = i0 + e - part * ng;
+        const double2 t = meet[part * cw + i];
+        const double f = BWD ? (double)wt[i] : 1.0;
+        v[h] += f * t.x;
+        v[2 + h] += f * t.y;
+      }
     }
-    u = warp_sum(u);
-    w = warp_sum(w);
+    warp_sums<4>(v);
     if (threadIdx.x % 32 == 0) {
-      double2* t = acc + 2 * (g - g0);
-      if (first_pass) {
-        t[0] = make_double2(u, w);
-        t[1] = make_double2(BWD ? 0.0 : (double)sm[i0], 0.0);
-      } else {
-        t[0].x += u;
-        t[0].y += w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t gh = g + h * FEAT_WARPS;
+        if (gh < ga || gh > gb) continue;
+        double2* t = acc + 2 * (gh - g0);
+        if (gh * a.Cg >= (uint32_t)c0) {
+          t[0] = make_double2(v[h], v[2 + h]);
+          t[1] = make_double2(BWD ? 0.0 : (double)sm[gh * a.Cg - (uint32_t)c0], 0.0);
+        } else {
+          t[0].x += v[h];
+          t[0].y += v[2 + h];
+        }
       }
     }
   }
@@ -1248,8 +1301,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
               __syncthreads();
             }
           }
-          last_sums<DT, VEC, ACT, DROP, BWD>(a, p, st, first, g0, gs, cp, sm, wt, meet, acc,
-                                             first_pass);
+          last_sums<DT, VEC, ACT, DROP, BWD>(a, p, st, first, g0, gs, cp, sm, wt, meet, acc);
           first_pass = false;
           if (p.c - p.tx * VEC + a.f.ncw * VEC >= p.c_end) break;
           p = last_next<VEC>(a.f, p);

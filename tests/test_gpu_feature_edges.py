@@ -93,6 +93,14 @@ def test_many_small_units(ba, shape, groups, layout):
     N._run(ba, shape, torch.float32, layout, groups, "silu")
 
 
+@pytest.mark.parametrize("dtype, shape, groups", [
+    (torch.bfloat16, (2, 2056, 1, 3, 3), 257), (torch.float32, (2, 1028, 2, 2, 3), 257),
+    (torch.bfloat16, (1, 8200, 1, 1, 3), 8), (torch.float32, (1, 1542, 1, 2, 2), 6)])
+def test_groups_that_begin_in_a_later_pass(ba, dtype, shape, groups):
+    """Rows wider than a pass of a thread block (256 accesses)."""
+    N._run(ba, shape, dtype, "last", groups, "silu")
+
+
 @pytest.mark.parametrize("layout", ["first", "last"])
 def test_launches_side_by_side(ba, layout):
     """Launches that fill the device and wait within themselves, from three
