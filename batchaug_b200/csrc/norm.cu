@@ -34,7 +34,8 @@ size_t norm_smem(const NormArgs& a, bool last, int32_t dtype, bool backward) {
   const size_t ring = f.vec == 1 ? 0 : FEAT_THREADS * bytes * 8 * (backward ? 2 : 1);
   const size_t cw = (size_t)f.ncw * f.vec;
   size_t n = std::max<size_t>(FEAT_THREADS, cw) * sizeof(double2) +
-             (size_t)a.ugroups * (2 * sizeof(double2) + sizeof(GroupStat)) + ring;
+             (size_t)a.ugroups * (2 * sizeof(double2) + sizeof(GroupStat)) + 2 * sizeof(Piece) +
+             ring;
   if (last)
     n += ((cw + 3) / 4 * 4 + std::max(5 * cw, (size_t)2 * FEAT_THREADS * f.vec)) * sizeof(float);
   return n;
@@ -59,8 +60,10 @@ int norm_occupancy(NormKernel fn, const NormKind& k, int32_t dtype, int32_t layo
     }
     c = held;
   }
-  // 227 KB a CTA at most and 228 KB an SM, 1 KB of it a CTA's own
-  return std::min<int>(c, std::max<int>(1, (int)(((size_t)228 << 10) / (smem + 1024))));
+  // 227 KB a CTA at most and 228 KB an SM, 1 KB of it a CTA's own; three rings
+  // cover the memory's latency, and a fourth CTA only adds partials (32 units
+  // of 8 MB: 153 us, with four 163)
+  return std::min<int>(std::min(c, 3), std::max<int>(1, (int)(((size_t)228 << 10) / (smem + 1024))));
 }
 
 // Column blocks (channels last): whole groups, whole columns, and at least 128
@@ -147,16 +150,21 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
     a.sets = (uint32_t)sets;
     a.wave = (uint32_t)wave;
   }
+  // pieces of the results (norm.cuh)
+  const bool whole = a.cluster || last;
+  a.sub_rows = whole ? f.rows : std::min<int64_t>(f.rows, NORM_PIECE * 256 * f.vec);
+  a.subs = (uint32_t)((f.rows + a.sub_rows - 1) / a.sub_rows);
 }
 
 struct NormScratch {
-  size_t done, part, chan, total;  // byte offsets; up to chan: zeroed
+  size_t done, ticket, part, chan, total;  // byte offsets; up to chan: zeroed
 };
 
 NormScratch norm_scratch(const NormArgs& a, bool backward) {
   NormScratch s;
   s.done = 0;
-  s.part = 16;
+  s.ticket = 16;
+  s.part = s.ticket + (a.subs > 1 ? align16(a.units * sizeof(uint32_t)) : 0);
   s.chan = s.part + (size_t)a.units * a.items * a.ugroups * sizeof(float4);
   s.total = s.chan +
             (backward ? align16((size_t)(a.f.B * a.f.C * a.f.nchunk) * sizeof(float2)) : 0);
@@ -259,6 +267,7 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
       (double)a.f.rows * (double)(d.layout == BA_CHANNELS_LAST ? a.Cg : (uint32_t)FEAT_WARPS);
   if (a.f.rows >= ((int64_t)1 << 31) || part_values >= 4294967296.0 ||
       (double)a.units * (double)a.items * FEAT_WARPS >= 4294967296.0 ||
+      (double)a.items * (double)a.subs >= 2147483648.0 ||
       (double)a.f.B * (double)a.f.nchunk >= 4294967296.0 || c.smem > (size_t)NORM_MAX_SMEM) {
     set_error("%s: tensor too large for one launch", what);
     return BA_EUNSUPPORTED;
@@ -277,6 +286,7 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   a.w_bf16 = d.param_dtype == BA_BF16;
   a.stats = d.stats;
   a.done = (uint32_t*)((char*)workspace + sc.done);
+  a.ticket = (uint32_t*)((char*)workspace + sc.ticket);
   a.part = (float4*)((char*)workspace + sc.part);
   a.chan = d.dweight || d.dbias ? (float2*)((char*)workspace + sc.chan) : nullptr;
   a.timeouts = wait_timeouts(cs);

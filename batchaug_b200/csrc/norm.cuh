@@ -22,9 +22,15 @@
 // counter, no fence, no second hop.  The sets' waves together are small
 // enough for their inputs to be in L2 still when the results read them again,
 // so HBM sees them once; where a unit alone is larger than that, the results
-// run backwards and find the end of it there.  A unit that eight CTAs can hold
-// is a cluster, whose barrier takes the place of the waiting: no zeroed words
-// and no cooperative launch, which is most of what a small call costs.
+// begin with the items' ends and find those there.  Channels first, the results
+// are taken in pieces of an item, first come, first served, the next piece's
+// loads behind those of the one at hand (32 units of 8 MB: 153 -> 124 us, with
+// the rings on whole lines).  Channels last, the same was slower (2x64x64^3
+// forward 41 -> 43 us, backward 64 -> 67; 2x32x128^3 145 -> 146, 233 -> 230), and
+// an item's results stay with its CTA.  (The sums' shares are the same every
+// time, so that the order of a sum is.)  A unit that eight CTAs can hold is a
+// cluster, whose barrier takes the place of the waiting: no zeroed words and no
+// cooperative launch, which is most of what a small call costs.
 //
 // A forward partial is the first and second moment about a value near the
 // mean, that value and the count; a thread sums about its own first value, and
@@ -39,6 +45,9 @@
 namespace ba {
 
 enum { ACT_NONE = 0, ACT_LEAKY = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+// Blocks of a piece of the results.
+constexpr int NORM_PIECE = 4;
 
 struct NormArgs {
   const void* x;
@@ -65,7 +74,10 @@ struct NormArgs {
   uint32_t items;  // work items of a unit
   uint32_t ugroups; // groups of a unit
   uint32_t sets;    // the CTAs are so many sets, each taking every sets-th wave
-  int32_t reverse; // results from the last voxel to the first
+  uint32_t subs;     // channels first: pieces of an item
+  int64_t sub_rows;  // voxels of a piece, of a channel
+  uint32_t* ticket;  // zeroed: those taken of each unit (subs > 1)
+  int32_t reverse;   // results from the last voxels of the items to the first
   int32_t cluster; // a unit is a thread block cluster (small units)
   double inv_n;    // 1 / values of a group
   float eps, slope;
@@ -522,6 +534,14 @@ struct Stream {
       x += span;
       dy += span;
     }
+  }
+  // after the current block comes the first one of `o`, of this many accesses
+  __device__ __forceinline__ int follow(const Stream& o) {
+    if constexpr (VEC > 1) {
+      x = o.x;
+      dy = o.dy;
+    }
+    return o.left;
   }
   // what the accesses lack that do not exist: zeros (a block ahead, like them)
   __device__ __forceinline__ void zero(int count) {
@@ -985,34 +1005,63 @@ __device__ __forceinline__ void last_apply(const NormArgs& a, const LastPlace& p
 // Channels first.  Item i of a group: 8 of its runs (channel, f.rows voxels),
 // one for each warp.  An access is 32 * VEC voxels of a warp.
 // ===========================================================================
-__device__ __forceinline__ void first_item(const NormArgs& a, uint32_t u, uint32_t i,
-                                           FirstPlace& p) {
+// A piece of a unit's results: piece j of item k, the ends first if reversed.
+struct Piece {
+  uint32_t k, j;
+  __device__ __forceinline__ bool is() const { return k != 0xFFFFFFFFu; }
+};
+__device__ __forceinline__ Piece piece_of(const NormArgs& a, uint32_t m) {
+  const uint32_t j = m / a.items;
+  return {j < a.subs ? m - j * a.items : 0xFFFFFFFFu, a.reverse ? a.subs - 1 - j : j};
+}
+
+// The next piece of unit u: asked for by thread 0 while the CTA works on one,
+// and read by all after the barrier behind it.
+struct Tickets {
+  Piece* slot;  // two in shared memory
+  uint32_t par;
+  __device__ __forceinline__ Piece take(const NormArgs& a, uint32_t u) const {
+    return piece_of(a, a.items + atomicAdd(a.ticket + u, 1u));
+  }
+};
+
+// The warp's voxels r .. r + n of its run.
+__device__ __forceinline__ void first_item(const NormArgs& a, uint32_t u, uint32_t i, int64_t r,
+                                           int64_t n, FirstPlace& p) {
   const uint32_t run = i * FEAT_WARPS + threadIdx.x / 32;
   const uint32_t cl = run / a.f.nchunk, k = run - cl * a.f.nchunk, b = u / a.G;
   p.lane = threadIdx.x % 32;
   p.b = b;
   p.k = k;
   p.c = (u - b * a.G) * a.Cg + cl;
-  p.s0 = k * a.f.rows;
-  p.n = cl < a.Cg ? (int)min(a.f.rows, a.f.S - p.s0) : 0;
+  p.s0 = k * a.f.rows + r;
+  p.n = cl < a.Cg ? (int)max((int64_t)0, min(min(n, a.f.rows - r), a.f.S - p.s0)) : 0;
   p.base = (p.b * a.f.C + p.c) * a.f.S + p.s0;
 }
+__device__ __forceinline__ void first_piece(const NormArgs& a, uint32_t u, Piece m,
+                                            FirstPlace& p) {
+  first_item(a, u, m.k, (int64_t)m.j * a.sub_rows, a.sub_rows, p);
+}
 
+template <int DT, int VEC, bool BWD>
+__device__ __forceinline__ void first_count(const FirstPlace& p, Stream<DT, VEC, BWD>& s) {
+  constexpr int every = 32 * VEC;
+  s.left = (p.n - first_at<VEC>(p.lane, 0) + every - 1) / every;  // towards zero: none below it
+  s.dec = 8;
+  s.blocks = (p.n + 8 * every - 1) / (8 * every);  // of the warp
+}
 template <int DT, int VEC, bool BWD>
 __device__ __forceinline__ Stream<DT, VEC, BWD> first_stream(const NormArgs& a,
                                                              const FirstPlace& p, char* ring) {
   Stream<DT, VEC, BWD> s;
   constexpr int every = 32 * VEC;  // voxels of a warp's access
-  const int own = first_at<VEC>(p.lane, 0);
-  const int64_t base = (p.base + own) * ESIZE<DT>;
+  const int64_t base = (p.base + first_at<VEC>(p.lane, 0)) * ESIZE<DT>;
   s.x = (const char*)a.x + base;
   s.dy = (const char*)a.dy + base;
   s.slot = ring + threadIdx.x * VEC * ESIZE<DT>;
   s.step = every * ESIZE<DT>;
   s.span = 8 * every * ESIZE<DT>;
-  s.left = (p.n - own + every - 1) / every;  // rounds towards zero: none below it
-  s.dec = 8;
-  s.blocks = (p.n + 8 * every - 1) / (8 * every);  // of the warp
+  first_count(p, s);
   return s;
 }
 
@@ -1154,73 +1203,101 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
   }
 }
 
+// y or dx of a piece whose first block is on its way, and of those that the CTA
+// draws.  A channel's constants go with the piece.
 template <int DT, int VEC, int ACT, int DROP, bool BWD>
-__device__ __forceinline__ void first_apply(const NormArgs& a, const FirstPlace& p,
-                                            Stream<DT, VEC, BWD>& st, const PairConst& k,
-                                            const DropRate& dr) {
-  if (p.n == 0) return;
+__device__ __forceinline__ void first_apply(const NormArgs& a, FirstPlace p,
+                                            Stream<DT, VEC, BWD>& st, uint32_t u, Tickets tk,
+                                            const GroupStat& gs, ChanParam cp, const DropRate& dr,
+                                            char* ring) {
   const float scale = DROP ? dr.scale : 1.0f;
-  char* out = (char*)a.out + (st.x - (const char*)a.x) - (VEC > 1 ? st.span : 0);
+  while (true) {
+    Piece next = {0xFFFFFFFFu, 0u}, after = next;
+    if (a.subs > 1) next = tk.slot[tk.par];
+    if (threadIdx.x == 0 && next.is()) after = tk.take(a, u);
+    const PairConst k = pair_const(gs, cp.w, cp.bias);
+    char* out = (char*)a.out + (st.x - (const char*)a.x) - (VEC > 1 ? st.span : 0);
 #pragma unroll 1
-  for (int q = 0; q < st.blocks; ++q, st.next(), out += st.span) {
-    const int more = q + 1 < st.blocks ? st.left - st.dec : 0;
-    const int s = (a.reverse ? st.blocks - 1 - q : q) * 8 * 32 * VEC;
-    st.fill();
-    if constexpr (VEC > 1) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        uint32_t keep[2];
-        if constexpr (DROP) first_block_keep<VEC, DROP>(a, dr, p, s + j * 32 * VEC, keep);
-        st.wait2();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          Raw<DT, VEC> vx = st.get_x(j + h), vd = {};
-          if constexpr (BWD) vd = st.get_dy(j + h);
-#pragma unroll
-          for (int i = 0; i < VEC / 2; i += 2) {
-            RawPair<DT> y0 = raw_pair<DT, VEC>(vx, i), y1 = raw_pair<DT, VEC>(vx, i + 1);
-            RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
-            const uint32_t w0 = DROP ? keep[h] << i : 0u, w1 = DROP ? keep[h] << (i + 1) : 0u;
-            if constexpr (BWD && DROP) {
-              d0 = pair_keep<DT, 1, 3>(d0, w0, w0);
-              d1 = pair_keep<DT, 1, 3>(d1, w1, w1);
-            }
-            norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d0, d1, k, k, a.slope, scale);
-            if constexpr (DROP && !BWD) {
-              y0 = pair_keep<DT, 1, 3>(y0, w0, w0);
-              y1 = pair_keep<DT, 1, 3>(y1, w1, w1);
-            }
-            raw_set_pair<DT, VEC>(vx, i, y0);
-            raw_set_pair<DT, VEC>(vx, i + 1, y1);
-          }
-          if (j + h < st.left) raw_store<DT, VEC>(out + (j + h) * 32 * VEC * ESIZE<DT>, vx);
+    for (int q = 0; q < st.blocks; ++q, st.next(), out += st.span) {
+      int more = st.left - st.dec;
+      if (q + 1 == st.blocks) {
+        more = 0;
+        if (next.is()) {
+          FirstPlace pn;
+          first_piece(a, u, next, pn);
+          more = st.follow(first_stream<DT, VEC, BWD>(a, pn, ring));
         }
-        st.issue2(more, j);
       }
-    } else {
-      uint32_t keep[8];
-      if constexpr (DROP) first_keep<VEC, DROP>(a.f, a.drop, dr, p, s, keep);
+      const int s = q * 8 * 32 * VEC;
+      st.fill();
+      if constexpr (VEC > 1) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        RawPair<DT> d[2] = {};
-        if constexpr (BWD) {
+        for (int j = 0; j < 8; j += 2) {
+          uint32_t keep[2];
+          if constexpr (DROP) first_block_keep<VEC, DROP>(a, dr, p, s + j * 32 * VEC, keep);
+          st.wait2();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
-            if constexpr (DROP)
-              d[h] = pair_keep<DT, 3, 3>(d[h], keep[j + 2 * h], keep[j + 2 * h + 1]);
+            Raw<DT, VEC> vx = st.get_x(j + h), vd = {};
+            if constexpr (BWD) vd = st.get_dy(j + h);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i += 2) {
+              RawPair<DT> y0 = raw_pair<DT, VEC>(vx, i), y1 = raw_pair<DT, VEC>(vx, i + 1);
+              RawPair<DT> d0 = raw_pair<DT, VEC>(vd, i), d1 = raw_pair<DT, VEC>(vd, i + 1);
+              const uint32_t w0 = DROP ? keep[h] << i : 0u, w1 = DROP ? keep[h] << (i + 1) : 0u;
+              if constexpr (BWD && DROP) {
+                d0 = pair_keep<DT, 1, 3>(d0, w0, w0);
+                d1 = pair_keep<DT, 1, 3>(d1, w1, w1);
+              }
+              norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d0, d1, k, k, a.slope, scale);
+              if constexpr (DROP && !BWD) {
+                y0 = pair_keep<DT, 1, 3>(y0, w0, w0);
+                y1 = pair_keep<DT, 1, 3>(y1, w1, w1);
+              }
+              raw_set_pair<DT, VEC>(vx, i, y0);
+              raw_set_pair<DT, VEC>(vx, i + 1, y1);
+            }
+            if (j + h < st.left) raw_store<DT, VEC>(out + (j + h) * 32 * VEC * ESIZE<DT>, vx);
           }
+          st.issue2(more, j);
         }
-        RawPair<DT> y0 = raw_join<DT>(st.rx[j], st.rx[j + 1]);
-        RawPair<DT> y1 = raw_join<DT>(st.rx[j + 2], st.rx[j + 3]);
-        norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d[0], d[1], k, k, a.slope, scale);
-        if constexpr (DROP && !BWD) {
-          y0 = pair_keep<DT, 3, 3>(y0, keep[j], keep[j + 1]);
-          y1 = pair_keep<DT, 3, 3>(y1, keep[j + 2], keep[j + 3]);
+      } else {
+        uint32_t keep[8];
+        if constexpr (DROP) first_keep<VEC, DROP>(a.f, a.drop, dr, p, s, keep);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          RawPair<DT> d[2] = {};
+          if constexpr (BWD) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              d[h] = raw_join<DT>(st.rd[j + 2 * h], st.rd[j + 2 * h + 1]);
+              if constexpr (DROP)
+                d[h] = pair_keep<DT, 3, 3>(d[h], keep[j + 2 * h], keep[j + 2 * h + 1]);
+            }
+          }
+          RawPair<DT> y0 = raw_join<DT>(st.rx[j], st.rx[j + 1]);
+          RawPair<DT> y1 = raw_join<DT>(st.rx[j + 2], st.rx[j + 3]);
+          norm_pairs<DT, ACT, DROP, BWD>(y0, y1, d[0], d[1], k, k, a.slope, scale);
+          if constexpr (DROP && !BWD) {
+            y0 = pair_keep<DT, 3, 3>(y0, keep[j], keep[j + 1]);
+            y1 = pair_keep<DT, 3, 3>(y1, keep[j + 2], keep[j + 3]);
+          }
+          single_store<DT>(out, 32 * ESIZE<DT>, j, st.left, y0, y1);
         }
-        single_store<DT>(out, 32 * ESIZE<DT>, j, st.left, y0, y1);
       }
     }
+    if (!next.is()) break;
+    first_piece(a, u, next, p);
+    if (VEC == 1 || st.blocks <= 0) {
+      st = first_stream<DT, VEC, BWD>(a, p, ring);
+      st.start();
+    } else {
+      first_count(p, st);
+    }
+    cp = chan_param(a, p.c, p.n > 0 ? a.f.C : 0);
+    if (threadIdx.x == 0) tk.slot[tk.par ^ 1] = after;
+    __syncthreads();
+    tk.par ^= 1;
   }
 }
 
@@ -1265,17 +1342,21 @@ static __device__ __forceinline__ void norm_param_grads(const NormArgs& a, doubl
 template <int DT, bool LAST, int VEC, int ACT, int DROP, bool BWD>
 __global__ void __launch_bounds__(FEAT_THREADS, 2)
     norm_kernel(const __grid_constant__ NormArgs a) {
-  // meet | group sums | group numbers | rings | weights | planes or constants
-  extern __shared__ double2 norm_smem[];
-  double2* meet = norm_smem;
+  // rings (whole lines: a warp's access is four of them, or five if they begin
+  // elsewhere) | meet | group sums | group numbers | tickets | weights | planes
+  // or constants
+  extern __shared__ __align__(128) char norm_smem[];
+  char* ring = norm_smem;
+  double2* meet = reinterpret_cast<double2*>(ring + RING_BYTES<DT, VEC, BWD>);
   double2* acc = meet + max(FEAT_THREADS, a.f.ncw * VEC);
   GroupStat* gs = reinterpret_cast<GroupStat*>(acc + 2 * a.ugroups);
-  char* ring = reinterpret_cast<char*>(gs + a.ugroups);
-  float* wt = reinterpret_cast<float*>(ring + RING_BYTES<DT, VEC, BWD>);
+  Piece* slot = reinterpret_cast<Piece*>(gs + a.ugroups);
+  float* wt = reinterpret_cast<float*>(slot + 2);
   float* sm = wt + (a.f.ncw * VEC + 3) / 4 * 4;
   const uint32_t waves = (a.units + a.wave - 1) / a.wave;
   const unsigned ctas = gridDim.x / (unsigned)a.sets;
   const unsigned set = blockIdx.x / ctas, own = blockIdx.x % ctas;
+  const Tickets tk = {slot, 0};
   int turn = 0;  // channels first: the part of `meet` that is free
   for (uint32_t w = set; w < waves; w += a.sets) {
     const uint32_t u0 = w * a.wave, total = min(a.wave, a.units - u0) * a.items;
@@ -1309,7 +1390,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
         last_put<BWD>(a, p, part, acc);
       } else {
         FirstPlace p;
-        first_item(a, u, i, p);
+        first_item(a, u, i, 0, a.f.rows, p);
         first_sums<DT, VEC, ACT, DROP, BWD>(a, u, p, ring, meet + turn * 2 * FEAT_WARPS, part);
         turn ^= 1;
       }
@@ -1343,17 +1424,20 @@ __global__ void __launch_bounds__(FEAT_THREADS, 2)
         }
       } else {
         FirstPlace p;
-        first_item(a, u, i, p);
+        first_piece(a, u, piece_of(a, i), p);
         Stream<DT, VEC, BWD> st = first_stream<DT, VEC, BWD>(a, p, ring);
-        if (a.reverse) st.turn();
         st.start();
         const ChanParam cp = chan_param(a, p.c, p.n > 0 ? a.f.C : 0);
         DropRate dr = {};
         if constexpr (DROP) dr = drop_rate(a.drop, p.b);
+        if (a.subs > 1) {
+          __syncthreads();  // the last use of the slots is over
+          if (threadIdx.x == 0) slot[0] = tk.take(a, u);
+        }
         GroupStat g;
         if (!norm_merge_one<BWD>(a, u, i == 0, meet + (4 + turn * 2) * FEAT_WARPS, g)) return;
         turn ^= 1;
-        first_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, pair_const(g, cp.w, cp.bias), dr);
+        first_apply<DT, VEC, ACT, DROP, BWD>(a, p, st, u, tk, g, cp, dr, ring);
       }
     }
   }
