@@ -10,12 +10,12 @@ namespace {
 
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-// Inputs of the sets' waves together.  L2 (126 MB, each of the two dies with
-// lines of its own) keeps about 32 MB of them from the sums to the results,
-// with the outputs' lines beside them: on 268 MB in units of 4 MB, the DRAM
-// reads of a forward pass were 269 MB with waves of 16 MB, 285 at 32 MB, 368 at
-// 48 MB and 451 at 64 MB.  But every wave waits once, and that costs more than
-// the reads: 182, 143, 148 and 139 us.
+// Inputs of the sets' waves together: 32 units of 8 MB took 135 us with waves
+// of 36 MB, 127 at 48, 124 at 72 and at 108, and 2x32x64^3 fp32 forward 40, 40,
+// 35 and 35 us.  L2 (126 MB, each of the two dies with lines of its own) keeps
+// about 32 MB of them from the sums to the results, with the outputs' lines
+// beside them, and larger waves read the rest again; but every wave waits once
+// and sums its threads' parts once, and that costs more than the reads.
 constexpr int64_t NORM_WAVE_BYTES = (int64_t)72 << 20;
 constexpr int64_t NORM_L2_BYTES = (int64_t)36 << 20;
 constexpr int NORM_MAX_SMEM = 227 << 10;
