@@ -207,7 +207,8 @@ def kernel_launches() -> int:
 
 def wait_status(device: torch.device | None = None) -> None:
     """Synchronise the current stream and raise if any bounded device wait
-    of the library (the TMA-staged resample's mbarrier waits) ran out."""
+    of the library (the TMA-staged resample's mbarrier waits, a group norm's
+    for the statistics) ran out."""
     dev = torch.device("cuda") if device is None else device
     check(lib.ba_wait_status(stream_ptr(dev)), "ba_wait_status")
 

@@ -113,9 +113,9 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   a.units = (uint32_t)units;
   const int64_t unit_bytes = f.S * (last ? f.width : a.Cg) * (d.dtype == BA_BF16 ? 2 : 4) *
                              (backward ? 2 : 1);
-  // two sets of CTAs, so that one streams while the other waits (units of
-  // 33 MB, forward: 41 us, 59 us with one set; four sets of smaller waves were
-  // no better)
+  // two sets of CTAs, so that one streams while the other waits (one set:
+  // 2x64x64^3 bf16 backward 86 us, not 65; 2x32x128^3 bf16 157 and 246 us, not 146
+  // and 233; four sets of smaller waves were no better)
   const int64_t sets = std::min<int64_t>(units, std::min<int64_t>(2, ctas / device_sms()));
   int64_t wave = std::min((units + sets - 1) / sets,
                           std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes / sets));

@@ -1339,6 +1339,15 @@ static __device__ __forceinline__ void norm_param_grads(const NormArgs& a, doubl
 }
 
 // ===========================================================================
+// The kernel.  Its floor is HBM, each tensor once.  Measured on the device:
+//   2x32x128^3 bf16, 8 groups, silu, last: 146 us forward, 234 backward; units of
+//     134 MB are read twice, 3 and 5 passes of 268 MB at 5.5 and 5.7 TB/s;
+//   8x4x128^3 fp32, 4 groups, first: 124 us (4.3 TB/s of input and output);
+//   2x64x64^3 bf16, 8 groups, silu, last: 41 and 64 us;
+//   2x48x96^3 bf16, 8 groups, gelu, dropout, last: 153 and 301 us, of 52 and 78
+//     at the floor: Philox and the normal distribution function bind;
+//   2x256x8^3 bf16, 32 groups, last: 10.4 us, latency.
+// Two CTAs an SM: eight channels' sums, constants and masks take 128 registers.
 template <int DT, bool LAST, int VEC, int ACT, int DROP, bool BWD>
 __global__ void __launch_bounds__(FEAT_THREADS, 2)
     norm_kernel(const __grid_constant__ NormArgs a) {
