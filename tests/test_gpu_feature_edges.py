@@ -93,6 +93,38 @@ def test_many_small_units(ba, shape, groups, layout):
     N._run(ba, shape, torch.float32, layout, groups, "silu")
 
 
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("shape, groups", [((1, 8, 40, 44, 48), 1), ((2, 6, 47, 53, 37), 2)])
+def test_units_of_many_thread_blocks(ba, shape, groups, p, dtype, layout):
+    """Above what a cluster takes: waiting launches, pieces of the results."""
+    N._run(ba, shape, dtype, layout, groups, "silu", p=p)
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_several_waves(ba, layout):
+    """85 MB of units in two waves and more, forward and backward, as the same
+    elements on their own.  |x - mean|, |xh| and |dy| are below 8 and rstd about 1,
+    so K is below 2e-4, dz within 8 (K + 16 u 9) < 2e-3, and dx, with the two
+    means' errors on top, within 2e-3 (1 + 1 + 8 8) < 0.14 of a value that a wrong
+    place would change by whole units; on average the errors are 2e-3 at most."""
+    shape = (6, 4, 96, 96, 96)
+    x = N._x(shape, torch.float32, layout).requires_grad_()
+    dy = N._x(shape, torch.float32, layout, seed=3)
+    y = ba.ops.group_norm(x, 4 if layout == "first" else 2, activation="silu", p=0.1, seed=2)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    assert float(dy.abs().max()) < 8
+    for b in range(6):
+        one = x.detach()[b:b + 1].clone(memory_format=torch.preserve_format).requires_grad_()
+        z = ba.ops.group_norm(one, 4 if layout == "first" else 2, activation="silu", p=0.1, seed=2,
+                              elem_offset=b)
+        (dz,) = torch.autograd.grad(z, one, dy[b:b + 1])
+        assert (y[b] - z[0]).abs().max() <= 2 * 1.2 * 1.13 * 2e-4
+        e = (dx[b] - dz[0]).abs()
+        assert e.max() <= 0.28 and e.mean() <= 4e-3
+
+
 @pytest.mark.parametrize("dtype, shape, groups", [
     (torch.bfloat16, (2, 2056, 1, 3, 3), 257), (torch.float32, (2, 1028, 2, 2, 3), 257),
     (torch.bfloat16, (1, 8200, 1, 1, 3), 8), (torch.float32, (1, 1542, 1, 2, 2), 6)])
