@@ -101,7 +101,14 @@ __global__ void __launch_bounds__(FEAT_THREADS)
   norm_param_grads<LAST>(a, meet);
 }
 
-// Units of at most so many bytes are clusters of up to eight CTAs.
+// Units of at most so many bytes are clusters of up to eight CTAs, if all of
+// them are resident at once (of fewer CTAs where there are many units).  bf16
+// with silu, forward and backward, clusters and waiting launches: 2x64x8^3 last
+// 10.4 and 12.3 us, 12.1 and 14.3; 2x64x12^3 last (216 KB) 10.3 and 12.3, 11.9 and
+// 14.6; 16x64x16^3 first (64 KB, 128 units) 12.4 and 10.2, 14.4 and 12.3, but 25 and
+// 37 with clusters of eight in more than one round.  At 512 KB they are even on
+// the device (2x64x16^3 last 12.4 and 12.5, 10.8 and 13.8), and the call is 2 us
+// shorter on the host.
 constexpr int64_t NORM_CLUSTER_BYTES = (int64_t)512 << 10;
 constexpr int NORM_CLUSTER = 8;
 
@@ -124,8 +131,9 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   a.sets = (uint32_t)sets;
   a.wave = (uint32_t)wave;
   a.reverse = sets * wave * unit_bytes > NORM_L2_BYTES;
+  const int64_t share = std::min<int64_t>(NORM_CLUSTER, ctas / units);
   ctas /= sets;
-  a.cluster = unit_bytes <= NORM_CLUSTER_BYTES;
+  a.cluster = unit_bytes <= NORM_CLUSTER_BYTES && share >= 1;
   if (a.cluster) {
     a.sets = 1;
     a.wave = (uint32_t)units;
@@ -138,8 +146,7 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   const int64_t least = last ? (int64_t)(FEAT_THREADS / f.ncw) * 8 : FEAT_TILE;
   int64_t parts = std::max<int64_t>(1, workers / (wave * rows_of_unit));
   if (a.cluster)
-    parts = last ? NORM_CLUSTER
-                 : std::max<int64_t>(1, (int64_t)NORM_CLUSTER * FEAT_WARPS / rows_of_unit);
+    parts = last ? share : std::max<int64_t>(1, share * FEAT_WARPS / rows_of_unit);
   parts = std::min(parts, (f.S + least - 1) / least);
   f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
   f.nchunk = (uint32_t)((f.S + f.rows - 1) / f.rows);
