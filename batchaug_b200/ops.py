@@ -13,6 +13,8 @@ import os
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib as L
 from . import _timing
@@ -410,6 +412,19 @@ def elastic_grid(shape, taps, magnitude, *, u=None, seed=0, elem_offset=0,
 # Feature maps: dropout and group norm (differentiable)
 # ---------------------------------------------------------------------------
 
+def _refuse_unseen(name: str, *args) -> None:
+    """Refuses a call that something watches which cannot see the launch behind
+    it: forward-mode differentiation would take the result for a constant, and
+    a recorded program (torch.jit.trace, make_fx) would return memory that
+    nobody wrote.  (functorch's transforms end at the tensors' addresses.)"""
+    if torch._C._get_tracing_state() is not None or get_proxy_mode() is not None:
+        raise NotImplementedError(f"{name} cannot be recorded by torch.jit.trace or make_fx")
+    if forward_ad._current_level >= 0:  # within dual_level()
+        for t in args:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def _feature_map(x: torch.Tensor, name: str):
     """``x`` dense in one of the two layouts the kernels take, and which: a
     (B,C,H,W,D) tensor contiguous as named or in torch.channels_last_3d is
@@ -502,6 +517,7 @@ class _Dropout(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, dy):
         desc, layout, tensors = ctx.call
+        _refuse_unseen("dropout", dy)
         if tensors:
             ctx.saved_tensors  # raises if one of them was written to since
         # the same draw on the gradient
@@ -512,8 +528,9 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
             channelwise: bool = False, rescale: bool = True) -> torch.Tensor:
     """Zero each voxel of x (B,C,H,W,D) with probability ``p`` and scale the
     others by 1 / (1 - p) (``rescale``); ``channelwise`` draws once for each
-    (element, channel).  Differentiable; the mask is never stored, the
-    backward pass draws it again.
+    (element, channel).  Differentiable (once, in reverse mode; forward mode and
+    a recorded call are refused); the mask is never stored, the backward pass
+    draws it again.
 
     ``p``: a number, or a (B,) tensor with a rate for each element.  ``mask``
     (B,): elements left as they are where false.  ``seed``: an integer, or a
@@ -522,6 +539,7 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     backward pass must see the value that the forward pass saw).  The bits
     depend on (seed, elem_offset + element, channel, voxel) only, not on
     the memory layout, which the result shares with x."""
+    _refuse_unseen("dropout", x, p)
     x, layout = _feature_map(x, "x")
     dtype = L.dtype_code(x)
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "dropout")
@@ -561,6 +579,7 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, dy):
+        _refuse_unseen("group_norm", dy)
         x, weight, bias, buf = ctx.saved_tensors[:4]
         desc, _, layout, _ = ctx.call
         desc = L.NormDesc.from_buffer_copy(desc)
@@ -604,7 +623,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     """dropout(activation(group_norm(x) * weight + bias)) of x (B,C,H,W,D),
     each group of C / num_groups consecutive channels of an element
     normalised by its own mean and biased variance.  Differentiable in x,
-    weight and bias.
+    weight and bias (once, in reverse mode; forward mode and a recorded call
+    are refused).
 
     ``activation``: None (or "none"), "relu", "leaky_relu" (with
     ``negative_slope``), "silu" or "gelu" (exact).  ``weight`` and ``bias``
@@ -612,6 +632,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     and ``elem_offset``: as in :func:`dropout`, rescaled; no dropout by
     default.  x may be contiguous or in torch.channels_last_3d, and the
     result is laid out as it is."""
+    _refuse_unseen("group_norm", x, weight, bias, p)
     x, layout = _feature_map(x, "x")
     dtype = L.dtype_code(x)
     num_groups = int(num_groups)

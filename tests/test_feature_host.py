@@ -158,3 +158,39 @@ def test_transform_params_on_the_host(ba):
     assert op.kind == L.BA_OP_DROPOUT and op.flags == L.BA_DROPOUT_CHANNEL
     assert op.seed == p["drop_seed"] and op.elem_offset == 4
     assert ba.NormalizeIntensityd(["x"], channel_wise=False).transform.channel_wise is False
+
+
+def _calls(ops, x, w):
+    return {"dropout": lambda: ops.dropout(x, 0.5, 1), "group_norm": lambda: ops.group_norm(x, 2),
+            "weight": lambda: ops.group_norm(torch.zeros(2, 4, 3, 3, 3), 2, w),
+            "rate": lambda: ops.dropout(torch.zeros(4, 2, 3, 3, 3), w, 1)}
+
+
+@pytest.mark.parametrize("name", ["dropout", "group_norm", "weight", "rate"])
+def test_forward_mode_is_refused(ba, name):
+    """A tangent that the launch would drop; without one the call goes on (and
+    ends at the CPU tensor)."""
+    from batchaug_b200 import ops
+    x, w = torch.zeros(2, 4, 3, 3, 3), torch.ones(4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _calls(ops, *dual)[name]()
+        with pytest.raises(ValueError, match="CUDA"):
+            _calls(ops, x, w)[name]()
+
+
+@pytest.mark.parametrize("name", ["dropout", "group_norm"])
+def test_a_recorded_call_is_refused(ba, name):
+    """Such a recording would hold the allocation and not the launch."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from batchaug_b200 import ops
+    x = torch.zeros(2, 4, 3, 3, 3)
+
+    def f(t):
+        return _calls(ops, t, None)[name]()
+    for record in (lambda: torch.jit.trace(f, (x,)), lambda: make_fx(f)(x),
+                   lambda: make_fx(f, pre_dispatch=True)(x)):
+        with pytest.raises(NotImplementedError, match="recorded"):
+            record()

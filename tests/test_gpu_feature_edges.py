@@ -201,3 +201,33 @@ def test_offsets_past_32_bits(ba, layout):
     K = 160 * N.U * 8 + 4 * N.U * 8 + 160 * N.U * 8
     y -= ref
     assert (y.abs_() <= 2 * K + 2 * N._half_step(torch.bfloat16) * (ref.abs_() + K)).all()
+
+
+@pytest.mark.parametrize("op", ["norm", "dropout"])
+def test_derivatives_that_would_be_lost_are_refused(ba, op):
+    """Forward mode over the call or over its gradient, and a recorded call; a
+    dual level without tangents, and a program compiled around the call, go on."""
+    fwd = torch.autograd.forward_ad
+
+    def f(t):
+        if op == "norm":
+            return ba.ops.group_norm(t, 2, activation="silu")
+        return ba.ops.dropout(t, 0.5, 3)
+
+    x = N._x((2, 8, 4, 5, 6), torch.float32, "last")
+    leaf = x.clone(memory_format=torch.preserve_format).requires_grad_()
+    y = f(leaf)
+    with fwd.dual_level():
+        one = torch.ones_like(x)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            f(fwd.make_dual(x, one))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            f(fwd.make_dual(leaf, one))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fwd.make_dual(one, one), retain_graph=True)
+        assert torch.equal(f(x), y)
+        torch.autograd.grad(y, leaf, one, retain_graph=True)
+    with pytest.raises(NotImplementedError, match="recorded"):
+        torch.jit.trace(f, (x,))
+    compiled = torch.compile(lambda t: f(t * 2.0) + 1.0, backend="eager")
+    assert torch.equal(compiled(x), f(x * 2.0) + 1.0)
