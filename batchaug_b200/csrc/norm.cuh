@@ -33,11 +33,18 @@
 // cooperative launch, which is most of what a small call costs.
 //
 // A forward partial is the first and second moment about a value near the
-// mean, that value and the count; a thread sums about its own first value, and
-// that shift is one of the summed values, so its distance from
-// the mean is itself part of the variance, and M2's relative error stays
-// below the number of values a thread sums times 2^-24, whatever the data's
-// offset.
+// mean, that value and the count.  A thread sums in fp32 about a centre: its
+// first value (channels first, the mean of its first access), and from then on
+// the mean of its values so far, taken after 1, 2 and 4 blocks of eight
+// accesses and after every fourth (`recentre`).  Sums about the first of n
+// values exceed M2 by a factor of n at most (it may be background, the others
+// not), those about the mean of as many values before them by 2.  With m <= 64
+// values to an accumulator between two centres (16 up to the first), its roundings
+// and those of the first moment make 3 m + 2 units: M2's relative error stays
+// below 8 * 50 * 2^-24, and 2^-24 more for each centre, whatever the data's offset
+// and order.  Where threads' sums meet, they are about a centre of theirs, or in
+// double.  (2x64x48^3 bf16 last, two centres a thread: 21.2 us, about the first
+// value alone 20.0; 2x32x128^3 and the channels-first volumes the same.)
 #pragma once
 
 #include "feature.cuh"
@@ -241,11 +248,29 @@ __device__ __forceinline__ void norm_add(RawPair<DT> x0, RawPair<DT> x1, RawPair
   q1 = fma2(g1, m1, q1);
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
+// After block q of a thread that has more of them.
+__device__ __forceinline__ bool recentres(int q) { return q < 2 || (q & 3) == 3; }
+
+// Forward: moves the centre to the mean of the thread's n values.  m2: their
+// second moment about the centre, without what is in s1; s0, their first moment,
+// keeps what the rounding of the new centre leaves.
+__device__ __forceinline__ void recentre(F2& nmean, F2& s0, F2& s1, F2& m2, float n) {
+  const F2 to = fma2(s0, f2(-rcp_hw(n)), nmean);
+  const F2 by = fma2(nmean, f2(-1.0f), to);  // the step, negated
+  const F2 left = fma2(by, f2(n), s0);
+  m2 = add2(m2, fma2(by, add2(s0, left), s1));
+  s0 = left;
+  s1 = f2(0.0f);
+  nmean = to;
 }
+// The same where the pair's halves are sums about one centre.
+__device__ __forceinline__ void recentre_one(F2& nmean, F2& s0, F2& s1, F2& m2, float n) {
+  s0 = f2(s0.x() + s0.y(), 0.0f);
+  s1 = f2(s1.x() + s1.y(), 0.0f);
+  recentre(nmean, s0, s1, m2, n);
+  nmean = f2(nmean.x());
+}
+
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -716,10 +741,10 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
   constexpr bool BLOCK = BWD && DROP != DROP_NONE;
   constexpr int NP = VEC > 1 ? VEC / 2 : 1;  // pairs of channels, or of rows
   if constexpr (BWD) st.zero(st.left);
-  F2 s0[NP], s1[NP];
+  F2 s0[NP], s1[NP], m2[NP];
   PairConst k[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) s0[i] = s1[i] = f2(0.0f);
+  for (int i = 0; i < NP; ++i) s0[i] = s1[i] = m2[i] = f2(0.0f);
   DropRate dr = {};
   if constexpr (BWD) {
     if constexpr (DROP) dr = drop_rate(a.drop, p.b);
@@ -727,7 +752,7 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
 #pragma unroll
     for (int i = 0; i < NP; ++i) k[i] = last_const<VEC, false>(a, p, i, sm);
   } else {
-    // the thread's first row is its shift
+    // the thread's first row is its first centre
 #pragma unroll
     for (int i = 0; i < NP; ++i) k[i] = {};
     if (st.left > 0) {
@@ -788,6 +813,18 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
         single_add<DT, ACT, BWD>(st, j, d, k[0], a.slope, s0[0], s1[0]);
       }
     }
+    if constexpr (!BWD) {
+      if (q + 1 < st.blocks && recentres(q)) {
+        const float n = (float)(8 * q + 8);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          if constexpr (VEC > 1)
+            recentre(k[i].nmean, s0[i], s1[i], m2[i], n);
+          else
+            recentre_one(k[i].nmean, s0[i], s1[i], m2[i], n);
+        }
+      }
+    }
   }
   // threads -> channels
   const int cw = a.f.ncw * VEC, rows = p.rows;
@@ -807,7 +844,7 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
         // a thread's (mean, M2); nothing when it had no row
         const float m = t * inv;
         u = m - (i & 1 ? k[h].nmean.y() : k[h].nmean.x());
-        w = __fmaf_rn(-t, m, w);
+        w = __fmaf_rn(-t, m, w + (i & 1 ? m2[h].y() : m2[h].x()));
       }
       us[i] = u;
       ws[i] = w;
@@ -826,9 +863,10 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
     }
   }
   __syncthreads();
-  // rows -> channel parts, about the mean of the group's first channel's first
-  // row (VEC rows at most, so in fp32: a conversion costs as much as four
-  // additions); then, a warp a group, -> groups, in double
+  // rows -> channel parts, about the mean of the part's first row (VEC rows at
+  // most, so in fp32: a conversion costs as much as four additions), and from
+  // there about that of the group's first channel's first row, in double; then,
+  // a warp a group, -> groups, in double
   const int parts = cw >= FEAT_THREADS ? 1 : FEAT_THREADS / cw;
   const int64_t c0 = p.c - p.tx * VEC;
   const int nch = (int)min((int64_t)cw, p.c_end - c0);  // channels of the pass
@@ -839,24 +877,32 @@ __device__ __forceinline__ void last_sums(const NormArgs& a, const LastPlace& p,
     const int part = parts == 1 ? 0 : (int)threadIdx.x / cw;
     const int ci = cb + (int)threadIdx.x - part * cw;
     if (part >= parts || ci >= nch) continue;
-    float u = 0.0f, w = 0.0f, k0 = 0.0f;
+    float u = 0.0f, w = 0.0f, k0 = 0.0f, kp = 0.0f, n = 0.0f;
     const uint32_t g = (uint32_t)(c0 + ci) / a.Cg;
     // about the first channel of the group, which an earlier pass may have had
-    if constexpr (!BWD)
+    if constexpr (!BWD) {
       k0 = g * a.Cg >= (uint32_t)c0 ? sm[g * a.Cg - (uint32_t)c0] : (float)acc[2 * (g - g0) + 1].x;
+      kp = part < rows ? sm[part * cw + ci] : k0;
+    }
 #pragma unroll 4
     for (int y = part; y < p.nty && (BWD || y < rows); y += parts) {
-      const float q = sm[y * cw + ci], m2 = plane[y * cw + ci];
+      const float q = sm[y * cw + ci], r = plane[y * cw + ci];
       if constexpr (BWD) {
         u += q;
-        w += m2;
+        w += r;
       } else {
-        const float d = q - k0, nd = (y < y1 ? rows1 : rows0) * d;
+        const float ny = y < y1 ? rows1 : rows0, d = q - kp, nd = ny * d;
+        n += ny;
         u += nd;
-        w += __fmaf_rn(nd, d, m2);
+        w += __fmaf_rn(nd, d, r);
       }
     }
     double2 t = make_double2((double)u, (double)w);
+    if constexpr (!BWD) {
+      const double d = (double)kp - (double)k0, nd = (double)n * d;
+      t.y += d * (2.0 * t.x + nd);
+      t.x += nd;
+    }
     if constexpr (BWD) {
       const double sc = DROP ? (double)dr.scale : 1.0;
       t.x *= sc;
@@ -1084,8 +1130,8 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
   const int cnt = max(st.left, 0) * VEC;  // the lane's voxels
   st.start();
   if constexpr (BWD) st.zero(st.left);
-  F2 s0 = f2(0.0f), s1 = f2(0.0f), u0 = f2(0.0f), u1 = f2(0.0f);
-  float shift = 0.0f, weight = 0.0f, rstd = 0.0f;
+  F2 s0 = f2(0.0f), s1 = f2(0.0f), u0 = f2(0.0f), u1 = f2(0.0f), m2 = f2(0.0f);
+  float weight = 0.0f, rstd = 0.0f;
   PairConst k = {};
   DropRate dr = {};
   if constexpr (BWD) {
@@ -1096,8 +1142,20 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
     rstd = t.y;
     if constexpr (DROP) dr = drop_rate(a.drop, p.b);
   } else {
-    if (cnt > 0) shift = load_f(first, DT, 0);
-    k.nmean = f2(-shift);
+    if (cnt > 0) {
+      if constexpr (VEC > 1) {  // the mean of the first access: exact for equal values
+        const Raw<DT, VEC> v = raw_load<DT, VEC>(first);
+        F2 t = add2(pair_value<DT>(raw_pair<DT, VEC>(v, 0)), pair_value<DT>(raw_pair<DT, VEC>(v, 1)));
+        if constexpr (VEC == 8)
+          t = add2(t, add2(pair_value<DT>(raw_pair<DT, VEC>(v, 2)),
+                           pair_value<DT>(raw_pair<DT, VEC>(v, 3))));
+        k.nmean = f2((t.x() + t.y()) * (-1.0f / VEC));
+      } else {
+        k.nmean = f2(-load_f(first, DT, 0));
+      }
+    } else {
+      k.nmean = f2(0.0f);
+    }
   }
 #pragma unroll 1
   for (int q = 0; q < st.blocks; ++q, st.next()) {
@@ -1148,11 +1206,20 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
         single_add<DT, ACT, BWD>(st, j, d, k, a.slope, s0, s1);
       }
     }
+    if constexpr (!BWD) {
+      // a block that another follows is whole in every lane
+      if (q + 1 < st.blocks && recentres(q)) {
+        s0 = add2(s0, u0);
+        s1 = add2(s1, u1);
+        u0 = u1 = f2(0.0f);
+        recentre_one(k.nmean, s0, s1, m2, (float)((q + 1) * 8 * VEC));
+      }
+    }
   }
   s0 = add2(s0, u0);
   s1 = add2(s1, u1);
-  // lanes -> run -> item, in double; forward, a lane's (mean, M2) about the
-  // first lane's shift, a run's about the first run's
+  // lanes -> run -> item, in double; forward, a lane's moments about the first
+  // lane's centre, a run's about the first run's
   double u, w, k0 = 0.0;
   if constexpr (BWD) {
     const double sc = DROP ? (double)dr.scale : 1.0;
@@ -1163,13 +1230,13 @@ __device__ __forceinline__ void first_sums(const NormArgs& a, uint32_t u_, const
     u *= (double)weight;
     w *= (double)weight;
   } else {
-    k0 = (double)__shfl_sync(0xFFFFFFFFu, shift, 0);
-    const double n = (double)cnt;
-    const float t0 = s0.x() + s0.y(), t1 = s1.x() + s1.y();
-    const float mt = cnt > 0 ? t0 / (float)cnt : 0.0f;
-    const double off = (double)shift - k0 + (double)mt;
-    u = warp_sum(cnt > 0 ? n * off : 0.0);
-    w = warp_sum(cnt > 0 ? (double)__fmaf_rn(-t0, mt, t1) + n * off * off : 0.0);
+    const float centre = -k.nmean.x();
+    k0 = (double)__shfl_sync(0xFFFFFFFFu, centre, 0);
+    const double t0 = (double)s0.x() + (double)s0.y();
+    const double t1 = (double)s1.x() + (double)s1.y() + (double)m2.x();
+    const double d = (double)centre - k0, nd = (double)cnt * d;
+    u = warp_sum(cnt > 0 ? t0 + nd : 0.0);
+    w = warp_sum(cnt > 0 ? t1 + d * (2.0 * t0 + nd) : 0.0);
   }
   const int warp = threadIdx.x / 32;
   if (p.lane == 0) {

@@ -4,6 +4,7 @@ gradients only, a first call under capture, launches side by side, offsets past
 32 bits, a great many small units.  Tolerances are test_gpu_group_norm's."""
 from __future__ import annotations
 
+import ctypes
 import os
 import subprocess
 import sys
@@ -231,3 +232,55 @@ def test_derivatives_that_would_be_lost_are_refused(ba, op):
         torch.jit.trace(f, (x,))
     compiled = torch.compile(lambda t: f(t * 2.0) + 1.0, backend="eager")
     assert torch.equal(compiled(x), f(x * 2.0) + 1.0)
+
+
+def _part_of_a_thread_block(x, groups, layout):
+    """Voxels of a thread block's (channels last) or a warp's part of the sums
+    of a single unit, from the size of the scratch: 16 bytes, 16 more with
+    pieces of results (channels first), and 16 for each part."""
+    from batchaug_b200 import _lib as L
+    B, C, H, W, D = x.shape
+    assert B == groups == 1
+    last = layout == "last"
+    desc = L.norm_desc(x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, B, C, H, W, D, groups, L.BA_F32,
+                       L.BA_CHANNELS_LAST if last else L.BA_CHANNELS_FIRST, L.BA_F32,
+                       L.BA_ACT_NONE, 1e-5, 0.0, 0.0, 0, 0, 0, 0, 0)
+    n = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 0) // 16 - (1 if last else 2)
+    parts, grain = (n, 8) if last else (n * 8 // C, 256)
+    return -(-(-(-H * W * D // parts)) // grain) * grain
+
+
+@pytest.mark.parametrize("layout, shape", [("last", (1, 512, 64, 64, 64)),
+                                           ("first", (1, 32, 128, 128, 128))])
+@pytest.mark.parametrize("noise", [0.0, 1.0])
+def test_variance_where_every_thread_begins_with_background(ba, layout, shape, noise):
+    """About 600 values a thread, its first ones 0 and the others 1001.3 or so:
+    sums about a thread's first value would be off by 600 times their own
+    errors.  With u = 2^-24: m values summed in fp32 about a centre of theirs have
+    an M2 within A (3 m + 2) u of itself, where A is the sum of squares over M2,
+    for the roundings of the sum, of the squares and of the first moment.  A
+    thread's first 8 values have m = 8 and A <= 8 (208 u; channels first 4
+    accumulators of 8 and an A of 32 / 4), later sums m <= 32 and A <= 2 (196 u),
+    each centre one u more (20 at most), and eight threads that meet 8 (3 8 + 2) u:
+    the variance within 440 u, and z within 220 u |z|, 4 u |z| for its own
+    roundings, plus test_gpu_group_norm's bound for the mean."""
+    x = torch.full(shape, 1001.3, device="cuda")
+    if noise:
+        x += noise * torch.randn(shape, generator=torch.Generator("cuda").manual_seed(1),
+                                 device="cuda")
+    if layout == "last":
+        x = x.contiguous(memory_format=torch.channels_last_3d)
+    S = shape[2] * shape[3] * shape[4]
+    part = _part_of_a_thread_block(x, 1, layout)
+    assert 400 * (2 if layout == "last" else 32) < part < 800 * (2 if layout == "last" else 32)
+    first = (torch.arange(S, device="cuda") % part) < (2 if layout == "last" else 128)
+    x.masked_fill_(first.view(1, 1, *shape[2:]), 0.0)
+    mean = x.double().mean()
+    d = x.double().sub_(mean)
+    rstd = 1 / torch.sqrt(d.square().mean() + 1e-5)
+    R, M = float(d.abs().max()), float(x.max())
+    z = d.mul_(rstd)
+    tol = float(rstd) * (160 * N.U * R + 4 * N.U * M) + 224 * N.U * z.abs()
+    y = ba.ops.group_norm(x, 1)
+    err = (y.double() - z).abs_().div_(tol)
+    assert float(err.max()) <= 1, float(err.max())
