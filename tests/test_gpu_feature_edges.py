@@ -284,3 +284,32 @@ def test_variance_where_every_thread_begins_with_background(ba, layout, shape, n
     y = ba.ops.group_norm(x, 1)
     err = (y.double() - z).abs_().div_(tol)
     assert float(err.max()) <= 1, float(err.max())
+
+
+def _line(ba, z_lo, z_hi, dtype, act, layout, n=1 << 16):
+    """(z, act(z)) along a line: x = z in that type, its mean and deviation put
+    back by bias and weight; z as the operator itself has it, unrounded in fp32."""
+    x = torch.linspace(z_lo, z_hi, n, device="cuda").to(dtype)
+    v = x.double()
+    w, b = ((t.float() * torch.ones(1 if layout == "first" else n, device="cuda"))
+            for t in (v.var(correction=0).sqrt(), v.mean()))
+    x = x.view(1, 1, n, 1, 1) if layout == "first" else x.view(1, n, 1, 1, 1)
+    if layout == "last":
+        x = x.contiguous(memory_format=torch.channels_last_3d)
+    z = ba.ops.group_norm(x.float(), 1, w, b, eps=0.0)
+    y = ba.ops.group_norm(x, 1, w, b, eps=0.0, activation=act)
+    return z.flatten().double(), y.flatten().double()
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gelu_keeps_the_digits_of_its_tail(ba, dtype, layout):
+    """With u = 2^-24: the tail's fit is within 2.8 u of its value (bf16: 78 u) and
+    its sum of products 6 u more, the reciprocal within 2 u, the exponential 4 u,
+    its argument (fp32: given back; bf16: z^2 u) and the last products 3 u: y
+    within 24 u (bf16: 100 u + z^2 u) of itself, and then a half step."""
+    z, y = _line(ba, -12.0, 12.0, dtype, "gelu", layout)
+    ref = z * 0.5 * torch.special.erfc(-z / 2**0.5)
+    rel = 24 * N.U if dtype == torch.float32 else (100 + z * z) * N.U + N._half_step(dtype)
+    err = (y - ref).abs() / (rel * ref.abs()).clamp(min=2.0**-126)
+    assert float(err.max()) <= 1, (float(err.max()), float(z[err.argmax()]))
