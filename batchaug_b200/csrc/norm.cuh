@@ -96,8 +96,9 @@ __device__ __forceinline__ float norm_param(const void* p, int bf16, int64_t c, 
 }
 
 // ---------------------------------------------------------------------------
-// Activations, on pairs.  exp2 and the reciprocal are the
-// hardware's (2 ulp), well below the outputs' tolerance in either type.  An SM
+// Activations, on pairs.  exp2 and the reciprocal are the hardware's, within 2^-22
+// and 2^-23 of their value: what an fp32 result is off by beside its own
+// rounding, and nothing in bf16.  An SM
 // makes 16 of them a clock, so they are what an activation costs.  (Sharing
 // one reciprocal among four values, 1/a = b (1/(a b)), took 3 to 7 % off a
 // forward pass with silu, but a value's last bit then depends on its
@@ -122,7 +123,18 @@ __device__ __forceinline__ F2 exp2_2(F2 t) { return f2(exp2_hw(t.x()), exp2_hw(t
 
 __device__ __forceinline__ F2 rcp2(F2 t) { return f2(rcp_hw(t.x()), rcp_hw(t.y())); }
 
+// 1 / (1 + exp(-z)).  The exponent's rounding is |z| 2^-24 of the exponential, which
+// for negative z is the value's own; FINE (fp32 results) gives it back to first
+// order.  Bf16 has no room for it, and a slope is a sum of order one.
+template <bool FINE>
 __device__ __forceinline__ F2 sigmoid2(F2 z) {
+  if constexpr (FINE) {
+    z = f2(min_nan(z.x(), 256.0f), min_nan(z.y(), 256.0f));  // 1 from 18 on, infinity too
+    const F2 c = f2(-1.44269504f), a = mul2(z, c);
+    F2 r = fma2(z, c, mul2(a, f2(-1.0f)));  // lost of the product and of the constant
+    r = fma2(z, f2(-1.9259630e-8f), r);
+    return rcp2(fma2(exp2_2(a), fma2(r, f2(0.69314718f), f2(1.0f)), f2(1.0f)));
+  }
   return rcp2(add2(exp2_2(mul2(z, f2(-1.44269504f))), f2(1.0f)));
 }
 
@@ -202,7 +214,7 @@ __device__ __forceinline__ F2 leaky2(F2 z, float slope) {
 template <int DT, int ACT>
 __device__ __forceinline__ F2 act_value2(F2 z, float slope) {
   if constexpr (ACT == ACT_LEAKY) return leaky2(z, slope);
-  if constexpr (ACT == ACT_SILU) return mul2(z, sigmoid2(z));
+  if constexpr (ACT == ACT_SILU) return mul2(z, sigmoid2<DT == BA_F32>(z));
   if constexpr (ACT == ACT_GELU) return gelu2<DT>(z);
   return z;
 }
@@ -211,7 +223,7 @@ __device__ __forceinline__ F2 act_slope2(F2 z, float slope) {
   if constexpr (ACT == ACT_LEAKY)
     return f2(z.x() > 0.0f ? 1.0f : slope, z.y() > 0.0f ? 1.0f : slope);
   if constexpr (ACT == ACT_SILU) {  // s + z s (1 - s)
-    const F2 s = sigmoid2(z);
+    const F2 s = sigmoid2<false>(z);
     return fma2(mul2(z, s), fma2(s, f2(-1.0f), f2(1.0f)), s);
   }
   if constexpr (ACT == ACT_GELU) {  // cdf + z pdf

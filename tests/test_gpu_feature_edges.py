@@ -313,3 +313,37 @@ def test_gelu_keeps_the_digits_of_its_tail(ba, dtype, layout):
     rel = 24 * N.U if dtype == torch.float32 else (100 + z * z) * N.U + N._half_step(dtype)
     err = (y - ref).abs() / (rel * ref.abs()).clamp(min=2.0**-126)
     assert float(err.max()) <= 1, (float(err.max()), float(z[err.argmax()]))
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_silu_far_below_zero(ba, dtype, layout):
+    """With u = 2^-24: the exponential within 4 u, its argument (fp32: given back, 2
+    u; bf16: |z| u), the sum 1 u, the reciprocal 2 u, the product 1 u, and then
+    a half step.  exp(80) is 5e34, so nothing leaves the range of fp32."""
+    z, y = _line(ba, -80.0, 80.0, dtype, "silu", layout)
+    ref = z / (1 + torch.exp(-z))
+    rel = 10 * N.U if dtype == torch.float32 else (8 + z.abs()) * N.U + N._half_step(dtype)
+    err = (y - ref).abs() / (rel * ref.abs()).clamp(min=2.0**-126)
+    assert float(err.max()) <= 1, (float(err.max()), float(z[err.argmax()]))
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "leaky_relu"])
+def test_activations_of_the_largest_values(ba, act, dtype, layout):
+    """A weight that takes z to the end of the type's range and past it: the far
+    ends of the activations are z (or infinity) and 0 (leaky: a hundredth)."""
+    x = N._x((1, 2, 4, 4, 4), dtype, layout)
+    y = ba.ops.group_norm(x, 1, torch.tensor([3e38, 1e20], device="cuda"), activation=act).double()
+    z = ba.ops.group_norm(x, 1, torch.tensor([3e38, 1e20], device="cuda")).double()
+    assert bool(torch.isinf(z).any())
+    up = z > 0
+    assert torch.equal(y[up], z[up])
+    low = y[~up & torch.isfinite(z)]
+    if act == "leaky_relu":
+        ref = 0.01 * z[~up & torch.isfinite(z)]
+        # the slope's and the product's roundings, and the type's on both sides
+        assert ((low - ref).abs() <= (4 * N.U + 2.1 * N._half_step(dtype)) * ref.abs()).all()
+    else:
+        assert not low.any()
