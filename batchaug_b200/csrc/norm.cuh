@@ -210,7 +210,7 @@ __device__ __forceinline__ F2 leaky2(F2 z, float slope) {
   return f2(z.x() < 0.0f ? n.x() : z.x(), z.y() < 0.0f ? n.y() : z.y());
 }
 
-// act(z) and act'(z)
+// act(z), and act'(z) of the smooth ones
 template <int DT, int ACT>
 __device__ __forceinline__ F2 act_value2(F2 z, float slope) {
   if constexpr (ACT == ACT_LEAKY) return leaky2(z, slope);
@@ -219,9 +219,7 @@ __device__ __forceinline__ F2 act_value2(F2 z, float slope) {
   return z;
 }
 template <int ACT>
-__device__ __forceinline__ F2 act_slope2(F2 z, float slope) {
-  if constexpr (ACT == ACT_LEAKY)
-    return f2(z.x() > 0.0f ? 1.0f : slope, z.y() > 0.0f ? 1.0f : slope);
+__device__ __forceinline__ F2 act_slope2(F2 z) {
   if constexpr (ACT == ACT_SILU) {  // s + z s (1 - s)
     const F2 s = sigmoid2<false>(z);
     return fma2(mul2(z, s), fma2(s, f2(-1.0f), f2(1.0f)), s);
@@ -232,6 +230,17 @@ __device__ __forceinline__ F2 act_slope2(F2 z, float slope) {
     return fma2(mul2(z, f2(0.39894228f)), e, c);
   }
   return f2(1.0f);
+}
+// The gradient of act at z for a gradient of g.
+template <int ACT>
+__device__ __forceinline__ F2 act_grad2(F2 g, F2 z, float slope) {
+  if constexpr (ACT == ACT_NONE) return g;
+  if constexpr (ACT == ACT_LEAKY) {
+    // slope 0: 0 whatever comes in, infinite ones included
+    const F2 n = slope == 0.0f ? f2(0.0f) : mul2(g, f2(slope));
+    return f2(z.x() > 0.0f ? g.x() : n.x(), z.y() > 0.0f ? g.y() : n.y());
+  }
+  return mul2(g, act_slope2<ACT>(z));
 }
 
 // ---------------------------------------------------------------------------
@@ -264,8 +273,8 @@ __device__ __forceinline__ void norm_pairs(RawPair<DT>& x0, RawPair<DT>& x1, Raw
   if constexpr (BWD) {
     F2 g0 = pair_value<DT>(d0), g1 = pair_value<DT>(d1);
     if constexpr (ACT != ACT_NONE) {
-      g0 = mul2(g0, act_slope2<ACT>(z0, slope));
-      g1 = mul2(g1, act_slope2<ACT>(z1, slope));
+      g0 = act_grad2<ACT>(g0, z0, slope);
+      g1 = act_grad2<ACT>(g1, z1, slope);
     }
     const F2 a0 = DROP ? mul2(k0.a, f2(scale)) : k0.a, a1 = DROP ? mul2(k1.a, f2(scale)) : k1.a;
     x0 = pair_raw<DT>(fma2(a0, g0, fma2(m0, k0.nc3, k0.nc2)));
@@ -294,8 +303,8 @@ __device__ __forceinline__ void norm_add(RawPair<DT> x0, RawPair<DT> x1, RawPair
     g0 = pair_value<DT>(d0);
     g1 = pair_value<DT>(d1);
     if constexpr (ACT != ACT_NONE) {
-      g0 = mul2(g0, act_slope2<ACT>(fma2(m0, k0.a, k0.bias), slope));
-      g1 = mul2(g1, act_slope2<ACT>(fma2(m1, k1.a, k1.bias), slope));
+      g0 = act_grad2<ACT>(g0, fma2(m0, k0.a, k0.bias), slope);
+      g1 = act_grad2<ACT>(g1, fma2(m1, k1.a, k1.bias), slope);
     }
   }
   p0 = add2(p0, g0);

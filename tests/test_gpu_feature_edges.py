@@ -347,3 +347,21 @@ def test_activations_of_the_largest_values(ba, act, dtype, layout):
         assert ((low - ref).abs() <= (4 * N.U + 2.1 * N._half_step(dtype)) * ref.abs()).all()
     else:
         assert not low.any()
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape, groups", [((2, 16, 6, 7, 8), 4), ((2, 6, 5, 5, 5), 3)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_rectified_values_stop_any_gradient(ba, bad, shape, groups, dtype, layout):
+    """An infinite or undefined gradient of a value that the rectifier has put to
+    zero counts as none, as in torch; one of a dropped value too."""
+    for p in (0.0, 0.4):
+        leaves = _leaves(N._x(shape, dtype, layout))
+        y = ba.ops.group_norm(leaves[0], groups, *leaves[1:], activation="relu", p=p, seed=3)
+        dy = N._x(shape, dtype, layout, seed=1)
+        dead = y.detach() == 0
+        assert bool(dead.any())
+        clean = torch.autograd.grad(y, leaves, dy.masked_fill(dead, 0.0), retain_graph=True)
+        got = torch.autograd.grad(y, leaves, dy.masked_fill(dead, bad))
+        assert all(torch.equal(a, c) for a, c in zip(got, clean))
