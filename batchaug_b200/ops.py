@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -470,13 +471,22 @@ def _drop_params(x: torch.Tensor, p, seed, name: str):
     return p, p_elem, int(seed) & 0xFFFFFFFFFFFFFFFF, seed_dev
 
 
+def _on_device(call):
+    """``call(x, ...)`` with x's device current: for the launch, and for the
+    query of its scratch, whose answer goes by the device."""
+    @functools.wraps(call)
+    def on(x, *args):
+        if x.device.index == torch._C._cuda_getDevice():  # current_device() without its checks
+            return call(x, *args)
+        with torch.cuda.device(x.device):
+            return call(x, *args)
+    return on
+
+
 def _launch(fn, name: str, passes: int, x: torch.Tensor, *args) -> None:
-    """One C entry on the current stream of x's device, with that device
-    current; ``passes``: how often it moves x's bytes."""
+    """One C entry on the current stream of x's device, which is current;
+    ``passes``: how often it moves x's bytes."""
     device = x.device
-    if device.index != torch._C._cuda_getDevice():  # current_device() without its checks
-        with torch.cuda.device(device):
-            return _launch(fn, name, passes, x, *args)
     if _timing._active is None:
         st = fn(*args, L.stream_ptr(device))
     else:
@@ -497,6 +507,7 @@ def _once_differentiable(backward):
     return call
 
 
+@_on_device
 def _dropout_call(x, desc):
     out = torch.empty_like(x)
     desc.src, desc.dst = x.data_ptr(), out.data_ptr()
@@ -555,16 +566,26 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     return _dropout_call(x, desc)
 
 
+@_on_device
 def _norm_forward(x, desc, groups):
     """y, and the buffer of the statistics (and, behind them, the scratch)."""
     y = torch.empty_like(x)
+    desc.out = y.data_ptr()
     size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 0)
     head = (x.shape[0] * groups * 8 + 15) & ~15
     buf = torch.empty(head + size, dtype=torch.uint8, device=x.device)
     at = buf.data_ptr()
-    desc.out, desc.stats = y.data_ptr(), at
+    desc.stats = at
     _launch(L.lib.ba_norm_forward, "ba_norm_forward", 2, x, ctypes.byref(desc), at + head, size)
     return y, buf
+
+
+@_on_device
+def _norm_backward(x, desc):
+    size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _launch(L.lib.ba_norm_backward, "ba_norm_backward", 3, x, ctypes.byref(desc), ws.data_ptr(),
+            size)
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -601,10 +622,7 @@ class _GroupNorm(torch.autograd.Function):
         if need_b:
             db = torch.empty_like(bias)
             desc.dbias = db.data_ptr()
-        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 1)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        _launch(L.lib.ba_norm_backward, "ba_norm_backward", 3, x, ctypes.byref(desc),
-                ws.data_ptr(), size)
+        _norm_backward(x, desc)
         return dx, dw, db, None
 
 

@@ -194,3 +194,41 @@ def test_a_recorded_call_is_refused(ba, name):
                    lambda: make_fx(f, pre_dispatch=True)(x)):
         with pytest.raises(NotImplementedError, match="recorded"):
             record()
+
+
+def test_queries_and_launches_are_made_on_the_tensors_device(ba, monkeypatch):
+    """The scratch of a call is asked for where the call is made, and with the
+    result's address in the descriptor (here another device than the current
+    one: the CPU, the library's calls replaced by records of it)."""
+    import contextlib
+
+    from batchaug_b200 import _lib as L
+    from batchaug_b200 import ops
+    current, calls = [], []
+
+    @contextlib.contextmanager
+    def device(d):
+        current.append(d)
+        yield
+        current.pop()
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(desc, *args):
+                calls.append((name, current[-1:], getattr(desc._obj, "out", 1)))
+                return 64 if name == "ba_norm_workspace_bytes" else 0
+            return call
+    x = torch.zeros(2, 4, 3, 3, 3, requires_grad=True)
+    monkeypatch.setattr(ops, "_feature_map", lambda t, name: (t, L.BA_CHANNELS_FIRST))
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice",
+                        lambda: current[-1].index if current else 0, raising=False)
+    monkeypatch.setattr(L, "stream_ptr", lambda d: 0)
+    monkeypatch.setattr(L, "lib", Lib())
+    w = torch.ones(4, requires_grad=True)
+    for y in (ops.group_norm(x, 2, w), ops.dropout(x, 0.5, 1)):
+        torch.autograd.grad(y, x, torch.ones_like(x))
+    assert [c[0] for c in calls] == ["ba_norm_workspace_bytes", "ba_norm_forward", "ba_dropout",
+                                     "ba_norm_workspace_bytes", "ba_norm_backward", "ba_dropout"]
+    assert all(c[1] == [x.device] and c[2] for c in calls), calls
+    assert not current
