@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(FEAT_THREADS, 3)
     Raw<DT, VEC> x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (r + j < p.rows) x[j] = raw_load<DT, VEC>(src + row_at(r + j, row));
+      if (r + j < p.rows) x[j] = raw_read<DT, VEC>(src + row_at(r + j, row));
     if (!a.channelwise) last_keep<VEC, KEYS>(a.f, a.drop, dr, p, r, keep);
     if constexpr (VEC > 1) {
 #pragma unroll

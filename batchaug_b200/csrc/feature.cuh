@@ -164,9 +164,15 @@ __device__ __forceinline__ RawPair<DT> pair_keep(RawPair<DT> p, uint32_t k0, uin
   }
 }
 
+// Of memory that nothing writes during the launch.
 template <int DT, int VEC>
 __device__ __forceinline__ Raw<DT, VEC> raw_load(const char* p) {
   return __ldg(reinterpret_cast<const Raw<DT, VEC>*>(p));
+}
+// Of memory that the launch may write (a result in place).
+template <int DT, int VEC>
+__device__ __forceinline__ Raw<DT, VEC> raw_read(const char* p) {
+  return *reinterpret_cast<const Raw<DT, VEC>*>(p);
 }
 template <int DT, int VEC>
 __device__ __forceinline__ void raw_store(char* p, const Raw<DT, VEC>& r) {
@@ -278,7 +284,7 @@ __device__ __forceinline__ void first_load(const char* x, int s, const FirstPlac
     for (int j = 0; j < 8; j += VEC) {
       const int at = s + first_at<VEC>(p.lane, j);
       if (at < p.n) {
-        const Raw<DT, VEC> r = raw_load<DT, VEC>(x + (int64_t)at * ESIZE<DT>);
+        const Raw<DT, VEC> r = raw_read<DT, VEC>(x + (int64_t)at * ESIZE<DT>);
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) t.p[j / 2 + i] = raw_pair<DT, VEC>(r, i);
       }
@@ -288,8 +294,8 @@ __device__ __forceinline__ void first_load(const char* x, int s, const FirstPlac
     for (int j = 0; j < 8; j += 2) {
       const int a0 = s + first_at<1>(p.lane, j), a1 = s + first_at<1>(p.lane, j + 1);
       Raw<DT, 1> v0 = 0, v1 = 0;
-      if (a0 < p.n) v0 = raw_load<DT, 1>(x + (int64_t)a0 * ESIZE<DT>);
-      if (a1 < p.n) v1 = raw_load<DT, 1>(x + (int64_t)a1 * ESIZE<DT>);
+      if (a0 < p.n) v0 = raw_read<DT, 1>(x + (int64_t)a0 * ESIZE<DT>);
+      if (a1 < p.n) v1 = raw_read<DT, 1>(x + (int64_t)a1 * ESIZE<DT>);
       t.p[j / 2] = raw_join<DT>(v0, v1);
     }
   }

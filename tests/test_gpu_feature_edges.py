@@ -365,3 +365,32 @@ def test_rectified_values_stop_any_gradient(ba, bad, shape, groups, dtype, layou
         clean = torch.autograd.grad(y, leaves, dy.masked_fill(dead, 0.0), retain_graph=True)
         got = torch.autograd.grad(y, leaves, dy.masked_fill(dead, bad))
         assert all(torch.equal(a, c) for a, c in zip(got, clean))
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 16, 8, 24, 20), (2, 3, 31, 33, 35), (3, 20, 9, 11, 13)])
+@pytest.mark.parametrize("flags", [0, 1, 2])
+def test_dropout_in_place(ba, shape, dtype, layout, flags):
+    """The C entry with dst == src (the Python function has a result of its own),
+    in a captured graph too: the second replay drops from what the first left."""
+    from batchaug_b200 import _lib as L
+    x = N._x(shape, dtype, layout)
+    B, C, H, W, D = shape
+    want = [ba.ops.dropout(x, 0.4, 7, channelwise=bool(flags & 1), rescale=bool(flags & 2))]
+    want.append(ba.ops.dropout(want[0], 0.4, 7, channelwise=bool(flags & 1),
+                               rescale=bool(flags & 2)))
+    v = x.clone(memory_format=torch.preserve_format)
+    d = L.dropout_desc(v.data_ptr(), v.data_ptr(), B, C, H, W, D, L.dtype_code(x),
+                       L.BA_CHANNELS_LAST if layout == "last" else L.BA_CHANNELS_FIRST, flags,
+                       0.4, 0, 0, 7, 0, 0)
+    L.check(L.lib.ba_dropout(ctypes.byref(d), L.stream_ptr(x.device)), "ba_dropout")
+    assert torch.equal(v, want[0])
+    v.copy_(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        L.check(L.lib.ba_dropout(ctypes.byref(d), L.stream_ptr(x.device)), "ba_dropout")
+    for w in want:
+        g.replay()
+        assert torch.equal(v, w)
