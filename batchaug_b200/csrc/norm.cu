@@ -101,16 +101,34 @@ __global__ void __launch_bounds__(FEAT_THREADS)
   norm_param_grads<LAST>(a, meet);
 }
 
-// Units of at most so many bytes are clusters of up to eight CTAs, if all of
-// them are resident at once (of fewer CTAs where there are many units).  bf16
-// with silu, forward and backward, clusters and waiting launches: 2x64x8^3 last
-// 10.4 and 12.3 us, 12.1 and 14.3; 2x64x12^3 last (216 KB) 10.3 and 12.3, 11.9 and
-// 14.6; 16x64x16^3 first (64 KB, 128 units) 12.4 and 10.2, 14.4 and 12.3, but 25 and
-// 37 with clusters of eight in more than one round.  At 512 KB they are even on
-// the device (2x64x16^3 last 12.4 and 12.5, 10.8 and 13.8), and the call is 2 us
-// shorter on the host.
+// Units of at most so many bytes are clusters of up to eight CTAs: as many as a
+// unit has of those that are resident at once, none where that is below one;
+// channels first, one for eight channels at least, so that groups of many channels
+// may need more than are resident, in rounds.  bf16 with silu, forward / backward
+// in us, clusters and waiting launches:
+//   2x64x8^3 last           9.0 / 14.1   12.3 / 18.0
+//   2x64x12^3 last          9.1 / 14.5   12.2 / 16.5   (216 KB)
+//   16x64x16^3 first        9.8 / 13.3   11.1 / 13.4   (64 KB, 128 units)
+//   16x64x12^3 first        9.7 / 12.5   10.5 / 12.8   (27 KB; clusters of eight, in
+//                                                      three rounds: 24.6 / 34.9)
+//   8x512x8^3, 32, first   13.8 / 21.9   17.0 / 21.5   (512 CTAs in clusters of two)
+//   16x512x8^3, 8, first   23.8 / 39.9   24.1 / 38.5   (1024 in clusters of eight)
+//   2x64x16^3 last         11.3 / 14.1   10.0 / 14.2   (512 KB)
+//   16x64x16^3 last        14.9 / 18.2   12.9 / 18.0   (512 KB)
+// and a cluster call is 2 us shorter on the host, so at 512 KB they are even.
 constexpr int64_t NORM_CLUSTER_BYTES = (int64_t)512 << 10;
 constexpr int NORM_CLUSTER = 8;
+
+// The items of a unit whose channels' voxels are cut into `parts`.
+void norm_cut(NormArgs& a, bool last, int64_t parts) {
+  Feat& f = a.f;
+  const int64_t grain = last ? 8 : FEAT_TILE;  // voxels: whole dropout blocks, whole tiles
+  const int64_t least = last ? (int64_t)(FEAT_THREADS / f.ncw) * 8 : FEAT_TILE;
+  parts = std::min(std::max<int64_t>(1, parts), (f.S + least - 1) / least);
+  f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
+  f.nchunk = (uint32_t)((f.S + f.rows - 1) / f.rows);
+  a.items = (uint32_t)(last ? f.nchunk : ((int64_t)a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
+}
 
 // Cuts the work for `ctas` resident CTAs: waves of units, items of a unit.
 void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ctas) {
@@ -120,42 +138,31 @@ void norm_schedule(NormArgs& a, const ba_norm_desc& d, bool backward, int64_t ct
   a.units = (uint32_t)units;
   const int64_t unit_bytes = f.S * (last ? f.width : a.Cg) * (d.dtype == BA_BF16 ? 2 : 4) *
                              (backward ? 2 : 1);
-  // two sets of CTAs, so that one streams while the other waits (one set:
-  // 2x64x64^3 bf16 backward 86 us, not 65; 2x32x128^3 bf16 157 and 246 us, not 146
-  // and 233; four sets of smaller waves were no better)
-  const int64_t sets = std::min<int64_t>(units, std::min<int64_t>(2, ctas / device_sms()));
-  int64_t wave = std::min((units + sets - 1) / sets,
-                          std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes / sets));
-  const int64_t waves = (units + wave * sets - 1) / (wave * sets) * sets;
-  wave = (units + waves - 1) / waves;
-  a.sets = (uint32_t)sets;
-  a.wave = (uint32_t)wave;
-  a.reverse = sets * wave * unit_bytes > NORM_L2_BYTES;
+  const int64_t rows_of_unit = last ? 1 : a.Cg;
   const int64_t share = std::min<int64_t>(NORM_CLUSTER, ctas / units);
-  ctas /= sets;
-  a.cluster = unit_bytes <= NORM_CLUSTER_BYTES && share >= 1;
+  if (unit_bytes <= NORM_CLUSTER_BYTES && share >= 1) {
+    norm_cut(a, last, last ? share : share * FEAT_WARPS / rows_of_unit);
+    a.cluster = a.items <= NORM_CLUSTER;
+  }
   if (a.cluster) {
     a.sets = 1;
     a.wave = (uint32_t)units;
     a.reverse = 0;
-  }
-  // parts of a channel's voxels, so that a wave has one item for each CTA
-  const int64_t grain = last ? 8 : FEAT_TILE;  // voxels: whole dropout blocks, whole tiles
-  const int64_t rows_of_unit = last ? 1 : a.Cg;
-  const int64_t workers = last ? ctas : ctas * FEAT_WARPS;
-  const int64_t least = last ? (int64_t)(FEAT_THREADS / f.ncw) * 8 : FEAT_TILE;
-  int64_t parts = std::max<int64_t>(1, workers / (wave * rows_of_unit));
-  if (a.cluster)
-    parts = last ? share : std::max<int64_t>(1, share * FEAT_WARPS / rows_of_unit);
-  parts = std::min(parts, (f.S + least - 1) / least);
-  f.rows = ((f.S + parts - 1) / parts + grain - 1) / grain * grain;
-  f.nchunk = (uint32_t)((f.S + f.rows - 1) / f.rows);
-  a.items = (uint32_t)(last ? f.nchunk : ((int64_t)a.Cg * f.nchunk + FEAT_WARPS - 1) / FEAT_WARPS);
-  // a group of more channels than a cluster has warps
-  if (a.cluster && a.items > NORM_CLUSTER) {
-    a.cluster = 0;
+  } else {
+    // two sets of CTAs, so that one streams while the other waits (one set:
+    // 2x64x64^3 bf16 backward 86 us, not 65; 2x32x128^3 bf16 157 and 246 us, not 146
+    // and 233; four sets of smaller waves were no better)
+    const int64_t sets = std::min<int64_t>(units, std::min<int64_t>(2, ctas / device_sms()));
+    int64_t wave = std::min((units + sets - 1) / sets,
+                            std::max<int64_t>(1, NORM_WAVE_BYTES / unit_bytes / sets));
+    const int64_t waves = (units + wave * sets - 1) / (wave * sets) * sets;
+    wave = (units + waves - 1) / waves;
     a.sets = (uint32_t)sets;
     a.wave = (uint32_t)wave;
+    a.reverse = sets * wave * unit_bytes > NORM_L2_BYTES;
+    // parts of a channel's voxels, so that a whole wave has one item for each CTA
+    const int64_t workers = ctas / sets * (last ? 1 : FEAT_WARPS);
+    norm_cut(a, last, workers / (wave * rows_of_unit));
   }
   // pieces of the results (norm.cuh)
   const bool whole = a.cluster || last;

@@ -232,3 +232,15 @@ def test_queries_and_launches_are_made_on_the_tensors_device(ba, monkeypatch):
                                      "ba_norm_workspace_bytes", "ba_norm_backward", "ba_dropout"]
     assert all(c[1] == [x.device] and c[2] for c in calls), calls
     assert not current
+
+
+def test_groups_too_wide_for_a_cluster_are_cut_for_the_device(ba):
+    """More channels than a cluster's 64 warps: the unit is cut into as many
+    parts as its channels have tiles of 256 voxels (eight tiles a part), not into
+    whole channels, as the size of the scratch shows (16 bytes and 16 a part)."""
+    from batchaug_b200 import _lib as L
+    for channels, n, tiles in ((128, 10, 4), (72, 8, 2), (256, 6, 1)):
+        d = _norm(L, batch=1, channels=channels, groups=1, H=n, W=n, D=n, dtype=L.BA_BF16,
+                  layout=L.BA_CHANNELS_FIRST)
+        size = L.lib.ba_norm_workspace_bytes(ctypes.byref(d), 0)
+        assert size == 16 + 16 * channels * tiles // 8

@@ -394,3 +394,13 @@ def test_dropout_in_place(ba, shape, dtype, layout, flags):
     for w in want:
         g.replay()
         assert torch.equal(v, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape, groups", [
+    ((1, 128, 10, 10, 10), 1), ((2, 72, 8, 8, 9), 1), ((2, 256, 6, 6, 7), 2),
+    ((20, 256, 4, 4, 4), 8), ((40, 64, 4, 4, 4), 1)])
+def test_groups_of_many_channels(ba, shape, groups, dtype):
+    """Channels first, more channels to a group than a cluster has warps, or as
+    many clusters as do not fit the device at once."""
+    N._run(ba, shape, dtype, "first", groups, "silu")
