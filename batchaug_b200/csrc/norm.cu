@@ -276,13 +276,18 @@ ba_status norm_run(const char* what, const ba_norm_desc* desc, bool backward, vo
   norm_plan(d, backward, c);
   NormArgs& a = c.a;
   const NormScratch& sc = c.scratch;
-  // counts are 32 bits: an item's rows, a partial's values, the items of a launch
+  // counts are 32 bits: an item's rows, a partial's values, the items of a launch;
+  // so are the bytes between a thread's rows (channels last)
+  const double row_step = d.layout == BA_CHANNELS_LAST
+                              ? (double)(FEAT_THREADS / a.f.ncw) * (double)d.channels * (double)esz
+                              : 0.0;
   const double part_values =
       (double)a.f.rows * (double)(d.layout == BA_CHANNELS_LAST ? a.Cg : (uint32_t)FEAT_WARPS);
   if (a.f.rows >= ((int64_t)1 << 31) || part_values >= 4294967296.0 ||
       (double)a.units * (double)a.items * FEAT_WARPS >= 4294967296.0 ||
       (double)a.items * (double)a.subs >= 2147483648.0 ||
-      (double)a.f.B * (double)a.f.nchunk >= 4294967296.0 || c.smem > (size_t)NORM_MAX_SMEM) {
+      (double)a.f.B * (double)a.f.nchunk >= 4294967296.0 || row_step >= 4294967296.0 ||
+      c.smem > (size_t)NORM_MAX_SMEM) {
     set_error("%s: tensor too large for one launch", what);
     return BA_EUNSUPPORTED;
   }

@@ -244,3 +244,21 @@ def test_groups_too_wide_for_a_cluster_are_cut_for_the_device(ba):
                   layout=L.BA_CHANNELS_FIRST)
         size = L.lib.ba_norm_workspace_bytes(ctypes.byref(d), 0)
         assert size == 16 + 16 * channels * tiles // 8
+
+
+def test_rows_too_long_for_a_stride_are_refused(ba):
+    """Channels last, a block of columns one access wide (the number of accesses
+    in a row has no small divisor): its threads are 256 rows apart, and 256 rows
+    of so many channels are 2^32 bytes."""
+    from batchaug_b200 import _lib as L
+    prime = 1048583
+    assert all(prime % k for k in range(2, 1025))
+    d = _norm(L, batch=1, channels=4 * prime, groups=4 * prime, H=2, W=1, D=1,
+              out=1 << 30, dy=1 << 32)
+    for fn in (L.lib.ba_norm_forward, L.lib.ba_norm_backward):
+        assert fn(ctypes.byref(d), 1 << 34, 1 << 40, None) == L.BA_EUNSUPPORTED
+        assert b"too large" in L.lib.ba_last_error()
+    # one row's bytes less
+    d.channels = d.groups = 4 * 1048573
+    assert L.lib.ba_norm_forward(ctypes.byref(d), None, 0, None) == L.BA_EINVAL
+    assert b"workspace" in L.lib.ba_last_error()
