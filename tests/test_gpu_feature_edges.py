@@ -13,6 +13,7 @@ import pytest
 import torch
 import torch.utils.checkpoint
 
+import feature_ref as R
 import test_gpu_group_norm as N
 
 pytestmark = pytest.mark.gpu
@@ -254,9 +255,9 @@ def _part_of_a_thread_block(x, groups, layout):
                                            ("first", (1, 32, 128, 128, 128))])
 @pytest.mark.parametrize("noise", [0.0, 1.0])
 def test_variance_where_every_thread_begins_with_background(ba, layout, shape, noise):
-    """About 600 values a thread, its first ones 0 and the others 1001.3 or so:
-    sums about a thread's first value would be off by 600 times their own
-    errors.  With u = 2^-24: m values summed in fp32 about a centre of theirs have
+    """About 300 (last) and 600 values a thread, its first ones 0 and the others
+    1001.3 or so: sums about a thread's first value would be off by so many times
+    their own errors.  With u = 2^-24: m values summed in fp32 about a centre of theirs have
     an M2 within A (3 m + 2) u of itself, where A is the sum of squares over M2,
     for the roundings of the sum, of the squares and of the first moment.  A
     thread's first 8 values have m = 8 and A <= 8 (208 u; channels first 4
@@ -404,3 +405,50 @@ def test_groups_of_many_channels(ba, shape, groups, dtype):
     """Channels first, more channels to a group than a cluster has warps, or as
     many clusters as do not fit the device at once."""
     N._run(ba, shape, dtype, "first", groups, "silu")
+
+
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_several_waves_against_the_definition(ba, layout):
+    """The 85 MB of test_several_waves in 64 bits on the device, every value
+    within test_gpu_group_norm's bounds (a thread sums 64 values or fewer here)."""
+    shape, groups = (6, 4, 96, 96, 96), 4 if layout == "first" else 2
+    x = N._x(shape, torch.float32, layout).requires_grad_()
+    dy = N._x(shape, torch.float32, layout, seed=3)
+    y = ba.ops.group_norm(x, groups, activation="silu")
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for b in range(shape[0]):
+        one = x.detach()[b:b + 1].double().contiguous().requires_grad_()
+        g = dy[b:b + 1].double()
+        ref, z = R.norm(one, groups, act="silu")
+        (ref_dx,) = torch.autograd.grad(ref, one, g)
+        ref, z = ref.detach(), z.detach()
+        K, rstd = N._bounds(one.detach(), groups, None, 1e-5, z)
+        tol = 1.13 * K + 16 * N.U * (ref.abs() + z.abs() + 1) + N._half_step(y.dtype) * ref.abs()
+        assert ((y.detach()[b:b + 1].double() - ref).abs() <= tol).all()
+        s = torch.sigmoid(z)
+        dz = g * (s + z * s * (1 - s))
+        e_dz = g.abs() * (K + 16 * N.U * (1 + z.abs()))
+        t1, t2 = dz.abs(), (dz * z).abs()
+        e1, e2 = e_dz + 80 * N.U * t1, e_dz * z.abs() + t1 * K + 80 * N.U * t2
+        m = {k: N._gmean(t, groups) for k, t in (("e1", e1), ("e2", e2), ("t1", t1), ("t2", t2))}
+        tol = rstd * (e_dz + m["e1"] + z.abs() * m["e2"] + K * m["t2"]
+                      + 176 * N.U * (t1 + m["t1"] + z.abs() * m["t2"])) \
+            + N._half_step(dx.dtype) * ref_dx.abs()
+        assert float(tol.mean()) < 1e-3
+        assert ((dx[b:b + 1].double() - ref_dx).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 6, 3, 6, 10), (1, 4, 2, 2, 33), (2, 8, 2, 9, 14)])
+def test_channels_that_end_within_a_dropout_block(ba, shape, dtype):
+    """Channels first, lengths of 8 k + 4: whole 16-byte accesses in fp32, the last
+    of them half a block of the generator."""
+    assert (shape[2] * shape[3] * shape[4]) % 8 == 4
+    N._run(ba, shape, dtype, "first", 2, "silu", p=0.3, seed=2**33 + 7)
+    x = N._x(shape, dtype, "first")
+    f = R.factor(shape, 0.3, 11).cuda()
+    y = ba.ops.dropout(x, 0.3, 11)
+    assert torch.equal(y == 0, f == 0)
+    ref = x.double() * f
+    # 1 - p, the reciprocal, the product, then the type's half step
+    assert ((y.double() - ref).abs() <= (4 * N.U + N._half_step(dtype)) * ref.abs()).all()
