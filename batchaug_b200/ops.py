@@ -9,12 +9,12 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import functools
 import os
 
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch._ops import _len_torch_dispatch_stack_pre_dispatch
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib as L
@@ -413,12 +413,18 @@ def elastic_grid(shape, taps, magnitude, *, u=None, seed=0, elem_offset=0,
 # Feature maps: dropout and group norm (differentiable)
 # ---------------------------------------------------------------------------
 
+# What _refuse_unseen looks into, and an ordinary call has none of: asked for in
+# line, 0.3 us of a call of 8
+_is_tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_modes_before_autograd = _len_torch_dispatch_stack_pre_dispatch
+
+
 def _refuse_unseen(name: str, *args) -> None:
     """Refuses a call that something watches which cannot see the launch behind
     it: forward-mode differentiation would take the result for a constant, and
     a recorded program (torch.jit.trace, make_fx) would return memory that
     nobody wrote.  (functorch's transforms end at the tensors' addresses.)"""
-    if torch._C._get_tracing_state() is not None or get_proxy_mode() is not None:
+    if _is_tracing() or get_proxy_mode() is not None:
         raise NotImplementedError(f"{name} cannot be recorded by torch.jit.trace or make_fx")
     if forward_ad._current_level >= 0:  # within dual_level()
         for t in args:
@@ -471,21 +477,10 @@ def _drop_params(x: torch.Tensor, p, seed, name: str):
     return p, p_elem, int(seed) & 0xFFFFFFFFFFFFFFFF, seed_dev
 
 
-def _on_device(call):
-    """``call(x, ...)`` with x's device current: for the launch, and for the
-    query of its scratch, whose answer goes by the device."""
-    @functools.wraps(call)
-    def on(x, *args):
-        if x.device.index == torch._C._cuda_getDevice():  # current_device() without its checks
-            return call(x, *args)
-        with torch.cuda.device(x.device):
-            return call(x, *args)
-    return on
-
-
 def _launch(fn, name: str, passes: int, x: torch.Tensor, *args) -> None:
-    """One C entry on the current stream of x's device, which is current;
-    ``passes``: how often it moves x's bytes."""
+    """One C entry on the current stream of x's device, which is current (it
+    answers for the query of a call's scratch too); ``passes``: how often it
+    moves x's bytes."""
     device = x.device
     if _timing._active is None:
         st = fn(*args, L.stream_ptr(device))
@@ -507,8 +502,10 @@ def _once_differentiable(backward):
     return call
 
 
-@_on_device
 def _dropout_call(x, desc):
+    if x.device.index != torch._C._cuda_getDevice():  # current_device() without its checks
+        with torch.cuda.device(x.device):
+            return _dropout_call(x, desc)
     out = torch.empty_like(x)
     desc.src, desc.dst = x.data_ptr(), out.data_ptr()
     _launch(L.lib.ba_dropout, "ba_dropout", 2, x, ctypes.byref(desc))
@@ -528,7 +525,8 @@ class _Dropout(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, dy):
         desc, layout, tensors = ctx.call
-        _refuse_unseen("dropout", dy)
+        if _is_tracing() or _modes() or _modes_before_autograd() or forward_ad._current_level >= 0:
+            _refuse_unseen("dropout", dy)
         if tensors:
             ctx.saved_tensors  # raises if one of them was written to since
         # the same draw on the gradient
@@ -550,25 +548,30 @@ def dropout(x: torch.Tensor, p, seed, *, mask=None, elem_offset: int = 0,
     backward pass must see the value that the forward pass saw).  The bits
     depend on (seed, elem_offset + element, channel, voxel) only, not on
     the memory layout, which the result shares with x."""
-    _refuse_unseen("dropout", x, p)
+    if _is_tracing() or _modes() or _modes_before_autograd() or forward_ad._current_level >= 0:
+        _refuse_unseen("dropout", x, p)
     x, layout = _feature_map(x, "x")
     dtype = L.dtype_code(x)
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "dropout")
     m = _dev_mask(mask, x.shape[0], x.device)
     flags = (L.BA_DROPOUT_CHANNEL if channelwise else 0) | (L.BA_DROPOUT_RESCALE if rescale else 0)
     B, C, H, W, D = x.shape
-    desc = L.dropout_desc(0, 0, B, C, H, W, D, dtype, layout, flags, p, L.ptr(p_elem) or 0,
-                          L.ptr(m) or 0, seed, L.ptr(seed_dev) or 0,
+    desc = L.dropout_desc(0, 0, B, C, H, W, D, dtype, layout, flags, p,
+                          0 if p_elem is None else p_elem.data_ptr(),
+                          0 if m is None else m.data_ptr(), seed,
+                          0 if seed_dev is None else seed_dev.data_ptr(),
                           int(elem_offset) & 0xFFFFFFFFFFFFFFFF)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, (desc, layout,
                                   [t for t in (p_elem, m, seed_dev) if t is not None]))
     return _dropout_call(x, desc)
 
 
-@_on_device
 def _norm_forward(x, desc, groups):
     """y, and the buffer of the statistics (and, behind them, the scratch)."""
+    if x.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
+            return _norm_forward(x, desc, groups)
     y = torch.empty_like(x)
     desc.out = y.data_ptr()
     size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 0)
@@ -580,8 +583,10 @@ def _norm_forward(x, desc, groups):
     return y, buf
 
 
-@_on_device
 def _norm_backward(x, desc):
+    if x.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
+            return _norm_backward(x, desc)
     size = L.lib.ba_norm_workspace_bytes(ctypes.byref(desc), 1)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     _launch(L.lib.ba_norm_backward, "ba_norm_backward", 3, x, ctypes.byref(desc), ws.data_ptr(),
@@ -600,7 +605,8 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, dy):
-        _refuse_unseen("group_norm", dy)
+        if _is_tracing() or _modes() or _modes_before_autograd() or forward_ad._current_level >= 0:
+            _refuse_unseen("group_norm", dy)
         x, weight, bias, buf = ctx.saved_tensors[:4]
         desc, _, layout, _ = ctx.call
         desc = L.NormDesc.from_buffer_copy(desc)
@@ -609,7 +615,8 @@ class _GroupNorm(torch.autograd.Function):
         # lies elsewhere, and may have lost its strides
         x = _like(x, x, layout)
         desc.x, desc.stats = x.data_ptr(), buf.data_ptr()
-        desc.weight, desc.bias = L.ptr(weight), L.ptr(bias)
+        desc.weight = None if weight is None else weight.data_ptr()
+        desc.bias = None if bias is None else bias.data_ptr()
         dy = _like(dy, x, layout)
         dx = dw = db = None
         desc.dy, desc.out = dy.data_ptr(), None
@@ -650,7 +657,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
     and ``elem_offset``: as in :func:`dropout`, rescaled; no dropout by
     default.  x may be contiguous or in torch.channels_last_3d, and the
     result is laid out as it is."""
-    _refuse_unseen("group_norm", x, weight, bias, p)
+    if _is_tracing() or _modes() or _modes_before_autograd() or forward_ad._current_level >= 0:
+        _refuse_unseen("group_norm", x, weight, bias, p)
     x, layout = _feature_map(x, "x")
     dtype = L.dtype_code(x)
     num_groups = int(num_groups)
@@ -670,14 +678,15 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, *, eps:
             raise ValueError(f"group_norm: weight is {weight.dtype}, bias {bias.dtype}")
     p, p_elem, seed, seed_dev = _drop_params(x, p, seed, "group_norm")
     B, C, H, W, D = x.shape
-    desc = L.norm_desc(x.data_ptr(), 0, 0, L.ptr(weight) or 0, L.ptr(bias) or 0, 0, 0, 0, B, C, H,
-                       W, D, num_groups, dtype, layout,
-                       L.BA_F32 if param is None else L.dtype_code(param),
-                       L.ACTIVATIONS[activation], eps, negative_slope, p, 0, L.ptr(p_elem) or 0,
-                       seed, L.ptr(seed_dev) or 0, int(elem_offset) & 0xFFFFFFFFFFFFFFFF)
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    desc = L.norm_desc(x.data_ptr(), 0, 0, 0 if weight is None else weight.data_ptr(),
+                       0 if bias is None else bias.data_ptr(), 0, 0, 0, B, C, H, W, D, num_groups,
+                       dtype, layout, L.BA_F32 if param is None else L.dtype_code(param),
+                       L.ACTIVATIONS[activation], eps, negative_slope, p, 0,
+                       0 if p_elem is None else p_elem.data_ptr(), seed,
+                       0 if seed_dev is None else seed_dev.data_ptr(),
+                       int(elem_offset) & 0xFFFFFFFFFFFFFFFF)
+    if (x.requires_grad or (weight is not None and weight.requires_grad)
+            or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         tensors = [t for t in (p_elem, seed_dev) if t is not None]
         return _GroupNorm.apply(x, weight, bias, (desc, num_groups, layout, tensors))
     return _norm_forward(x, desc, num_groups)[0]
