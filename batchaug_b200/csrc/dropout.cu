@@ -15,8 +15,9 @@ struct DropoutArgs {
 
 // 8 rows of the thread's columns a pass, each channel's bits from one block, so
 // that a block's eight decisions stay in the thread that drew them.  2x64x64^3
-// bf16 at p = 0.1: 35 us, 3.8 TB/s of 6.5; the integer units bind (a block is 60
-// operations for 8 values): ALU 58 % and issue slots 69 % busy.
+// bf16 at p = 0.1: 33 us, 4.1 TB/s of 6.5; the integer units bind (a block is 60
+// operations for 8 values): ALU 59 % and issue slots 68 % busy.  The bound of three
+// CTAs an SM (80 registers) costs 44 bytes of spill stores there.
 template <int DT, int VEC, int KEYS>
 __global__ void __launch_bounds__(FEAT_THREADS, 3)
     dropout_last(const __grid_constant__ DropoutArgs a) {
@@ -67,9 +68,10 @@ __global__ void __launch_bounds__(FEAT_THREADS, 3)
 
 // A warp a run of a channel, four tiles of 256 voxels in flight; a lane's 16
 // bytes of bf16 are one dropout block (fp32: words handed over between lanes).
-// 16x4x128^3 bf16, a rate for each element: 109 us, 4.9 TB/s, the integer units
-// 66 to 70 % busy (87 operations for 8 values, where HBM leaves time for 89).
-// 2x3x91x109x91 fp32, where no vector width divides a channel: 12.5 us, 3.5 TB/s.
+// 16x4x128^3 bf16, a rate for each element: 107 us, 5.0 TB/s, the integer units
+// 66 % busy (87 operations for 8 values, where HBM leaves time for 89).
+// 2x3x91x109x91 fp32, where no vector width divides a channel: 11.9 us, 3.6 TB/s
+// (bf16 there takes 174 registers, one CTA an SM).
 template <int DT, int VEC, int KEYS>
 __global__ void __launch_bounds__(FEAT_THREADS)
     dropout_first(const __grid_constant__ DropoutArgs a) {

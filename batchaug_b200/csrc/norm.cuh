@@ -28,9 +28,11 @@
 // the rings on whole lines).  Channels last, the same was slower (2x64x64^3
 // forward 41 -> 43 us, backward 64 -> 67; 2x32x128^3 145 -> 146, 233 -> 230), and
 // an item's results stay with its CTA.  (The sums' shares are the same every
-// time, so that the order of a sum is.)  A unit that eight CTAs can hold is a
-// cluster, whose barrier takes the place of the waiting: no zeroed words and no
-// cooperative launch, which is most of what a small call costs.
+// time, so that the order of a sum is.)  A unit of up to 512 KB is a cluster of up
+// to eight CTAs, unless there are more units than resident CTAs, or (channels
+// first) more than 64 channels in a group: its barrier takes the place of the
+// waiting, so no zeroed words and no cooperative launch, which is most of what a
+// small call costs.
 //
 // A forward partial is the first and second moment about a value near the
 // mean, that value and the count.  A thread sums in fp32 about a centre: its
@@ -44,7 +46,10 @@
 // below 8 * 50 * 2^-24, and 2^-24 more for each centre, whatever the data's offset
 // and order.  Where threads' sums meet, they are about a centre of theirs, or in
 // double.  (2x64x48^3 bf16 last, two centres a thread: 21.2 us, about the first
-// value alone 20.0; 2x32x128^3 and the channels-first volumes the same.)
+// value alone 20.0; 2x32x128^3 and the channels-first volumes the same.)  The
+// backward sums have no centre: fp32 over a thread's part, within as many units of
+// 2^-24 of their terms' magnitudes as it has values (up to some hundreds at the
+// sizes measured), and double from there.
 #pragma once
 
 #include "feature.cuh"
@@ -1472,14 +1477,16 @@ static __device__ __forceinline__ void norm_param_grads(const NormArgs& a, doubl
 
 // ===========================================================================
 // The kernel.  Its floor is HBM, each tensor once.  Measured on the device:
-//   2x32x128^3 bf16, 8 groups, silu, last: 146 us forward, 234 backward; units of
-//     134 MB are read twice, 3 and 5 passes of 268 MB at 5.5 and 5.7 TB/s;
-//   8x4x128^3 fp32, 4 groups, first: 124 us (4.3 TB/s of input and output);
-//   2x64x64^3 bf16, 8 groups, silu, last: 41 and 64 us;
-//   2x48x96^3 bf16, 8 groups, gelu, dropout, last: 153 and 301 us, of 52 and 78
-//     at the floor: Philox and the normal distribution function bind;
-//   2x256x8^3 bf16, 32 groups, last: 10.4 us, latency.
-// Two CTAs an SM: eight channels' sums, constants and masks take 128 registers.
+//   2x32x128^3 bf16, 8 groups, silu, last: 143 us forward, 236 backward; units of
+//     134 MB are read twice, 3 and 5 passes of 268 MB at 5.6 and 5.7 TB/s;
+//   8x4x128^3 fp32, 4 groups, first: 121 us (4.5 TB/s of input and output);
+//   2x64x64^3 bf16, 8 groups, silu, last: 40 and 64 us;
+//   2x48x96^3 bf16, 8 groups, gelu, dropout, last: 152 and 300 us, of 52 and 78
+//     at the floor: Philox and the normal distribution function, and latency;
+//   2x256x8^3 bf16, 32 groups, last: 9.5 us, latency.
+// Two CTAs an SM: eight channels' sums, constants and masks take 128 registers,
+// and with dropout more (bf16 last, bytes of spill stores: 24 forward, backward 40
+// to 76; without dropout the backward pass spills 12 with silu, 20 with gelu).
 template <int DT, bool LAST, int VEC, int ACT, int DROP, bool BWD>
 __global__ void __launch_bounds__(FEAT_THREADS, 2)
     norm_kernel(const __grid_constant__ NormArgs a) {
